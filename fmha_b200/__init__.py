@@ -9,6 +9,9 @@ binding raises.
 
 Layout (the reference's Q/O layout, with K/V in [B,H,S,D]):
   Q [B, Hq, 1, D] bf16, K/V [B, Hkv, S, D] bf16, O [B, Hq, 1, D] fp16.
+
+Serving with a paged cache: ``fmha_rope_append``, ``fmha_paged_decode`` and
+``fmha_prompt`` (serving.py).
 """
 from __future__ import annotations
 
@@ -17,7 +20,7 @@ from ._lib import (FMHA_ERR_CUDA, FMHA_ERR_DEVICE_TIMEOUT, FMHA_ERR_INVALID_ARG,
                    VARIANT_BULK, VARIANT_LDG, VARIANTS, FmhaError, check, load, status_string)
 
 __all__ = ["fmha_forward", "fmha_forward_ptr", "fmha_forward_varlen_ptr", "seqlens_poisson", "fill_normal_bf16", "device_error", "FmhaError",
-           "load", "version"]
+           "load", "version", "fmha_rope_append", "fmha_paged_decode", "fmha_paged_decode_workspace", "fmha_prompt"]
 
 TENSOR_Q, TENSOR_K, TENSOR_V = 1, 2, 3
 
@@ -123,3 +126,15 @@ def device_error() -> int:
 
 def version() -> str:
     return load().fmha_version().decode()
+
+
+
+_SERVING = ("fmha_rope_append", "fmha_paged_decode", "fmha_paged_decode_workspace", "fmha_prompt")
+
+
+def __getattr__(name):  # serving.py needs torch; the rest of this module does not
+    if name in _SERVING:
+        from . import serving
+        globals().update({n: getattr(serving, n) for n in _SERVING})
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -19,6 +19,7 @@
 
 #include "../../include/fmha.h"
 #include "decode_common.cuh"
+#include "serving.hpp"
 
 namespace fmha {
 
@@ -80,6 +81,18 @@ fmha_status_t device_info(DeviceInfo* out) {
   return FMHA_OK;
 }
 
+}  // namespace
+
+fmha_status_t serving_device(ServingDevice* out) {
+  DeviceInfo d;
+  const fmha_status_t st = device_info(&d);
+  if (st != FMHA_OK) return st;
+  out->sms = d.sms;
+  out->smem_optin = d.smem_optin;
+  out->err = d.err;
+  return FMHA_OK;
+}
+
 // Sets the kernel's dynamic shared-memory limit once per (kernel, device).
 fmha_status_t ensure_smem(const void* fn, int bytes) {
   int dev = 0;
@@ -94,6 +107,8 @@ fmha_status_t ensure_smem(const void* fn, int bytes) {
   g_smem_set.insert(key);
   return FMHA_OK;
 }
+
+namespace {
 
 fmha_status_t blocks_per_sm(const void* fn, int threads, int* out) {
   int dev = 0;

@@ -1,0 +1,105 @@
+// serving.hpp -- what the paged-cache entry points (rope_append.cu,
+// paged_decode.cu, prompt.cu) share on the host: device facts kept by
+// fmha_api.cu, argument checks, and the launch with programmatic overlap.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <cmath>
+#include <cstdlib>
+
+#include "../../include/fmha.h"
+
+namespace fmha {
+
+struct ServingDevice {
+  int sms = 0;
+  int smem_optin = 0;
+  unsigned int* err = nullptr;  // device error word
+};
+
+// Facts of the current device, and a kernel's dynamic shared-memory limit set
+// to `bytes` once per device (both in fmha_api.cu).
+fmha_status_t serving_device(ServingDevice* out);
+fmha_status_t ensure_smem(const void* fn, int bytes);
+
+// Device error sites of the serving kernels (bits 8..15 of the error word).
+enum : unsigned {
+  kSiteAppendPosition = 16,  // a new token's position or length is impossible
+  kSiteAppendPage = 17,      // its page number is outside the pool
+  kSiteDecodeLength = 18,
+  kSiteDecodePage = 19,
+  kSitePromptLength = 20,
+  kSitePromptWait = 21  // a bounded wait ran out
+};
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+inline fmha_status_t check_heads(int hq, int hkv, int d) {
+  if (hq <= 0 || hkv <= 0 || d <= 0 || hq % hkv != 0) return FMHA_ERR_INVALID_ARG;
+  if (d != 128 && d != 256) return FMHA_ERR_UNSUPPORTED;
+  if (hq > 65535) return FMHA_ERR_UNSUPPORTED;
+  return FMHA_OK;
+}
+
+// A [tokens, heads, d] operand of 16-bit elements.
+inline fmha_status_t check_rows(const void* p, int64_t stride, int64_t heads, int d) {
+  if (!p || stride < heads * d) return FMHA_ERR_INVALID_ARG;
+  if (!aligned16(p) || stride % 8 != 0) return FMHA_ERR_MISALIGNED;
+  return FMHA_OK;
+}
+
+// The cache, for sequences whose Q has type `dtype`. Strides along axes of
+// one element are put to what they would be in a dense page.
+inline fmha_status_t check_cache(const fmha_paged_cache_t* in, int hkv, int d, int dtype,
+                                 fmha_paged_cache_t* out) {
+  if (!in) return FMHA_ERR_INVALID_ARG;
+  fmha_paged_cache_t c = *in;
+  if (!c.k || !c.v || !c.block_table || !c.seqlens_kv) return FMHA_ERR_INVALID_ARG;
+  if (c.num_pages <= 0 || c.page_size <= 0 || c.max_pages <= 0) return FMHA_ERR_INVALID_ARG;
+  if (c.dtype != dtype && c.dtype != FMHA_DTYPE_E4M3) return FMHA_ERR_UNSUPPORTED;
+  if (c.page_size == 1) c.token_stride = d;
+  if (hkv == 1) c.head_stride = d;
+  if (c.num_pages == 1) c.page_stride = 0;
+  if (c.page_stride < 0 || c.head_stride < d || c.token_stride < d || c.table_stride < 0)
+    return FMHA_ERR_INVALID_ARG;
+  if (!(c.k_scale > 0.0f) || !(c.v_scale > 0.0f) || std::isinf(c.k_scale) || std::isinf(c.v_scale))
+    return FMHA_ERR_INVALID_ARG;
+  if (c.dtype != FMHA_DTYPE_E4M3 && (c.k_scale != 1.0f || c.v_scale != 1.0f))
+    return FMHA_ERR_INVALID_ARG;
+  const int per16 = c.dtype == FMHA_DTYPE_E4M3 ? 16 : 8;
+  if (!aligned16(c.k) || !aligned16(c.v)) return FMHA_ERR_MISALIGNED;
+  if (c.page_stride % per16 || c.head_stride % per16 || c.token_stride % per16)
+    return FMHA_ERR_MISALIGNED;
+  if ((reinterpret_cast<uintptr_t>(c.block_table) | reinterpret_cast<uintptr_t>(c.seqlens_kv)) & 3u)
+    return FMHA_ERR_MISALIGNED;
+  *out = c;
+  return FMHA_OK;
+}
+
+// Launches with programmatic stream serialization: the kernel may start while
+// the one before it in the stream finishes, and waits in
+// grid_dependency_wait() before it touches memory.
+template <class Prm>
+inline fmha_status_t launch_serving(void (*fn)(const Prm), dim3 grid, unsigned block, size_t smem,
+                                    cudaStream_t stream, const Prm& P) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  const char* const plain = std::getenv("FMHA_NO_PDL");
+  cfg.numAttrs = plain && std::atoi(plain) ? 0 : 1;
+  if (cudaLaunchKernelEx(&cfg, fn, P) != cudaSuccess) {
+    cudaGetLastError();
+    return FMHA_ERR_CUDA;
+  }
+  return FMHA_OK;
+}
+
+}  // namespace fmha

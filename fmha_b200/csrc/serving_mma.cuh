@@ -1,0 +1,106 @@
+// serving_mma.cuh -- device pieces shared by the serving kernels: 16-byte
+// asynchronous copies, ldmatrix, the 16x8x16 MMA on bf16 or fp16 operands
+// with fp32 accumulators, and the roundings between them.
+//
+// MMA fragments (lane = 4*g + c, g = 0..7, c = 0..3): A[16x16] holds rows g
+// and g+8 at columns 2c, 2c+1 (a0, a1) and 2c+8, 2c+9 (a2, a3); B[16x8] holds
+// rows 2c, 2c+1 (b0) and 2c+8, 2c+9 (b1) of column g; C[16x8] holds row g
+// (c0, c1) and row g+8 (c2, c3) at columns 2c, 2c+1.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "decode_common.cuh"
+
+namespace fmha {
+
+// 16 bytes global -> shared; `bytes` = 0 reads nothing and fills with zeros.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+template <bool BF16>
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                      uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Two fp32 values rounded to 16 bits each (x in the low half).
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&p);
+  } else {
+    const __half2 p = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&p);
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (BF16) return make_float2(bf_lo(w), bf_hi(w));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// Two weights x, y >= 0 as the sum of two 16-bit pairs: `hi` cuts them off
+// towards zero, `lo` rounds what that left (together about twice the bits).
+// Both parts have the weight's sign and `lo` is never zero (at least the
+// type's smallest number, 2^-126 or 2^-24), so that an infinite value keeps
+// its sign and does not meet a zero: hi*inf + lo*inf = inf.
+template <bool BF16>
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  constexpr float kLeast = BF16 ? 0x1p-126f : 0x1p-24f;
+  if constexpr (BF16)
+    hi = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+  else
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y), "f"(x));
+  const float2 h = unpack2<BF16>(hi);
+  lo = pack2<BF16>(fmaxf(x - h.x, kLeast), fmaxf(y - h.y, kLeast));
+}
+
+// Two e4m3 codes (low 16 bits) as two fp16 values: exact.
+__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t codes) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}"
+      : "=r"(r)
+      : "r"(codes));
+  return r;
+}
+
+}  // namespace fmha

@@ -160,6 +160,133 @@ fmha_status_t fmha_forward_noalloc(const void* Q, const void* K, const void* V,
                                    int num_heads_kv, int seqlen_kv,
                                    int head_dim, fmha_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Serving with a paged KV cache: fmha_rope_append fills the pages,
+ * fmha_paged_decode attends over them with one new token per sequence, and
+ * fmha_prompt attends over whole packed prompts. No reference counterpart:
+ * the reference's cache holds at most 16 dense rows.
+ *
+ * Conventions beyond the ones above:
+ *  - head_dim is 128 or 256; any num_heads_q that is a multiple of
+ *    num_heads_kv;
+ *  - `dtype` names the type of Q, K and V (bf16 or fp16), `o_dtype` that of O
+ *    (fp16 or bf16);
+ *  - Q, K, V and O rows are [tokens, heads, head_dim] with adjacent heads; the
+ *    `*_stride` arguments are elements from one token to the next (at least
+ *    heads * head_dim, a multiple of 8), so views of a fused projection work;
+ *  - rows that see no key (an empty sequence, a causal row before the first
+ *    key) get O = 0 and LSE = -infinity;
+ *  - lengths, offsets and page numbers are device memory, so they are checked
+ *    by the kernels: a sequence with an impossible length, or a token whose
+ *    page number or position is out of range, is left out and reported
+ *    through fmha_device_error (FMHA_ERR_INVALID_ARG); nothing is read or
+ *    written out of bounds;
+ *  - softmax_scale == 0 means 1/sqrt(head_dim); a negative, NaN or infinite
+ *    scale is rejected.
+ */
+
+/* Element types. */
+typedef enum {
+  FMHA_DTYPE_BF16 = 0,
+  FMHA_DTYPE_FP16 = 1,
+  FMHA_DTYPE_E4M3 = 2 /* cache pages only */
+} fmha_dtype_t;
+
+/* A paged KV cache and the sequences in it. Token j of sequence b, kv head h
+ * lies at
+ *   k + block_table[b*table_stride + j/page_size] * page_stride
+ *     + h*head_stride + (j%page_size)*token_stride      (elements; v alike)
+ * with head_dim adjacent elements, so pages may be stored head by head or
+ * token by token, and k and v may be parts of one allocation. Strides are
+ * multiples of 16 bytes. With FMHA_DTYPE_E4M3 pages an element stands for
+ * code * k_scale (v_scale); with 16-bit pages, which have the type of Q, both
+ * scales must be 1. */
+typedef struct fmha_paged_cache {
+  void* k;
+  void* v;
+  const int32_t* block_table; /* [batch, max_pages], device memory */
+  const int32_t* seqlens_kv;  /* [batch], device memory: tokens of each sequence */
+  int64_t page_stride;
+  int64_t head_stride;
+  int64_t token_stride;
+  int64_t table_stride; /* elements between block_table rows */
+  int32_t num_pages;    /* pages in the pool */
+  int32_t page_size;    /* tokens in a page, any number >= 1 */
+  int32_t max_pages;    /* block_table columns */
+  int32_t dtype;        /* fmha_dtype_t of the pages */
+  float k_scale;
+  float v_scale;
+} fmha_paged_cache_t;
+
+/*
+ * fmha_rope_append -- rotates the new tokens' queries and keys by their
+ * positions and writes the new keys and values into the cache, in one pass:
+ *   Q [total_tokens, num_heads_q, head_dim], K, V [total_tokens, num_heads_kv,
+ *   head_dim]; sequence b's new tokens are rows cu_seqlens_q[b] ..
+ *   cu_seqlens_q[b+1]-1 (device int32 [batch+1]), or row b alone when
+ *   cu_seqlens_q is null (then total_tokens == batch). seqlens_kv counts the
+ *   tokens of each sequence with the new ones, so the last new token has
+ *   position seqlens_kv[b] - 1.
+ *   cos_table, sin_table [max_position, rotary_dim/2] fp32. The first
+ *   rotary_dim elements of a head (0: none; a multiple of 16) are turned in
+ *   pairs (i, i + rotary_dim/2), or (2i, 2i+1) when `interleaved`:
+ *     y1 = x1*cos - x2*sin,  y2 = x2*cos + x1*sin     (fp32, rounded once)
+ * Writes Q_out (the rotated queries; may be Q itself with the same stride),
+ * the cache rows (rotated keys; values as they are; for e4m3 pages divided by
+ * the scale, and saturated), and, unless null, K_out (the rotated keys,
+ * packed, for fmha_prompt; may be K itself). Rows behind the last sequence
+ * are left as they were. Two new tokens must not map to one cache row.
+ */
+fmha_status_t fmha_rope_append(const void* Q, const void* K, const void* V, void* Q_out,
+                               void* K_out, const fmha_paged_cache_t* cache,
+                               const int32_t* cu_seqlens_q, const float* cos_table,
+                               const float* sin_table, int total_tokens, int batch,
+                               int num_heads_q, int num_heads_kv, int head_dim,
+                               int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                               int64_t q_out_stride, int64_t k_out_stride, int rotary_dim,
+                               int max_position, int interleaved, int dtype,
+                               fmha_stream_t stream);
+
+/* Bytes of device scratch that fmha_paged_decode needs for these heads (the
+ * same for every batch and length); -1 for sizes it does not support. */
+int64_t fmha_paged_decode_workspace(int num_heads_q, int num_heads_kv, int head_dim);
+
+/*
+ * fmha_paged_decode -- attention of one new token per sequence over the
+ * paged cache:
+ *   O[b,h,:] = softmax(softmax_scale * Q[b,h,:] . K_b[:,kvh,:]^T) . V_b[:,kvh,:]
+ *   Q [batch, num_heads_q, head_dim], O the same in o_dtype;
+ *   LSE [batch, num_heads_q] fp32 or null: the natural logarithm of the sum
+ *   of exp(scaled score).
+ * workspace: at least fmha_paged_decode_workspace(...) bytes, 16-byte
+ * aligned, overwritten; calls that may run at the same time (two streams, two
+ * captured graphs) need one each. It holds nothing between calls. The launch
+ * depends on no length, so a captured call may be replayed as sequences grow.
+ */
+fmha_status_t fmha_paged_decode(const void* Q, const fmha_paged_cache_t* cache, void* O,
+                                float* LSE, int batch, int num_heads_q, int num_heads_kv,
+                                int head_dim, int64_t q_stride, int64_t o_stride,
+                                float softmax_scale, int dtype, int o_dtype, void* workspace,
+                                int64_t workspace_bytes, fmha_stream_t stream);
+
+/*
+ * fmha_prompt -- attention over packed prompts of different lengths:
+ *   Q [total_q, num_heads_q, head_dim], K, V [total_kv, num_heads_kv,
+ *   head_dim], O [total_q, num_heads_q, head_dim] in o_dtype;
+ *   LSE [total_q, num_heads_q] fp32 or null.
+ * Sequence b's queries are rows cu_seqlens_q[b] .. cu_seqlens_q[b+1]-1, its
+ * keys rows cu_seqlens_kv[b] .. cu_seqlens_kv[b+1]-1 (device int32
+ * [batch+1]; cu_seqlens_kv null: the same as cu_seqlens_q). With `causal`,
+ * query i of nq sees keys j <= i + (nk - nq): the last query sees every key.
+ * Rows behind the last sequence are left as they were.
+ */
+fmha_status_t fmha_prompt(const void* Q, const void* K, const void* V, void* O, float* LSE,
+                          const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_kv,
+                          int total_q, int total_kv, int batch, int num_heads_q,
+                          int num_heads_kv, int head_dim, int64_t q_stride, int64_t k_stride,
+                          int64_t v_stride, int64_t o_stride, float softmax_scale, int causal,
+                          int dtype, int o_dtype, fmha_stream_t stream);
+
 /* Human-readable name of a status code (static storage). Reference
  * counterpart: the HIP_CHECK error text (fmha_host.cpp:26-35). */
 const char* fmha_status_string(fmha_status_t status);
