@@ -1,14 +1,40 @@
 // prompt.cu -- fmha_prompt: attention over packed prompts of different
-// lengths, causal or not, with grouped query heads.
+// lengths, causal or not, with grouped query heads, on the tcgen05 tensor
+// cores.
 //
-// Mathematics: per query row one pass over the keys with the running maximum
-// m and sum l of 2^(s - m), s = scale*log2(e) * q.k, and o = sum 2^(s - m) v
-// (fp32); O = o / l.
+// Mathematics: per query row one pass over the keys with a reference maximum
+// m and the sum l of 2^(s - m), s = scale*log2(e) * q.k, and o = sum
+// 2^(s - m) v (fp32); O = o / l. m follows the running maximum only when that
+// has risen by more than kSlack (a factor of 2^8 in the weights, which fp32
+// sums and 16-bit weights bear): o, which lies in tensor memory, is then
+// rescaled, and otherwise left alone.
 //
-// Split: a CTA takes 64 query rows of one (sequence, head), 16 to a warp, and
-// walks the sequence's keys in tiles through a two-stage cp.async ring.
+// Split. A tile is 128 rows: 128/PACK tokens of PACK query heads that share
+// their kv head (PACK: the largest power of two in G), so short prompts fill
+// tiles too. Keys come in blocks of 128. At head_dim 128 a CTA takes two
+// tiles side by side, so that the tensor cores work on one while the softmax
+// warps are busy with the other; at 256 one tile, whose output takes the
+// tensor memory of two, with the scores double-buffered instead.
+//
+// Warps: 4 per tile for the softmax (one thread per row: a row's maximum and
+// sum need no shuffles), one to issue TMA loads (a ring of 32 KB stages: 128
+// keys x 128 columns of K or V), one to issue the MMAs. S (128 fp32 columns)
+// and P (64 columns of 16-bit pairs, over S) stay in tensor memory; P is the
+// A operand of P.V from there.
+//
+// Precision: P is rounded to the operands' type, except that bf16 operands
+// with an fp16 result take P as two bf16 parts and a second P.V product, so
+// that the result deserves its 11 bits. l sums the weights before rounding.
+//
+// Masked places: scores behind a row's last key are replaced, whatever they
+// are. V rows behind the sequence's end are zeroed in shared memory. A V
+// element that is NaN or infinite inside the sequence, but behind a row's
+// last key, would still meet that row's zero weight in the tensor core; a row
+// whose output shows a NaN that its weights do not explain is computed again
+// on the CUDA cores over its own keys.
 #include <cuda_runtime.h>
 
+#include <cfloat>
 #include <cmath>
 #include <cstring>
 
@@ -16,11 +42,13 @@
 #include "decode_common.cuh"
 #include "serving.hpp"
 #include "serving_mma.cuh"
+#include "tcgen05.cuh"
 
 namespace fmha {
 namespace {
 
 struct PromptParams {
+  CUtensorMap map_q, map_k, map_v;
   const uint16_t* q;
   const uint16_t* k;
   const uint16_t* v;
@@ -32,29 +60,52 @@ struct PromptParams {
   int64_t q_stride, k_stride, v_stride, o_stride;
   float scale_log2;
   int causal;
+  int pack_log2;  // PACK
   int o_bf16;
   unsigned int* err;
 };
 
-constexpr int kRowsQ = 64;
-constexpr int kPromptThreads = 128;
+constexpr int kTileRows = 128;
+constexpr int kKeys = 128;                 // keys of a block
+constexpr int kStageBytes = kKeys * 256;   // 128 keys x 128 columns
+constexpr int kBlockBytes = kKeys * 128;   // 128 rows x 64 columns
+constexpr float kSlack = 8.0f;
 
 template <int D>
 struct PromptShape {
-  static constexpr int kKeys = D == 128 ? 64 : 32;
-  static constexpr int kRow = D * 2;
-  static constexpr int kQ = kRowsQ * kRow;
-  static constexpr int kKV = kKeys * kRow;
-  static constexpr int kSmem = kQ + 4 * kKV;
+  static constexpr int kTiles = D == 128 ? 2 : 1;    // query tiles of a CTA
+  static constexpr int kHalves = D / 128;            // 128-column parts of a head
+  static constexpr int kSoftWarps = 4 * kTiles;
+  static constexpr int kThreads = 32 * (kSoftWarps + 2);
+  static constexpr int kQBytes = 2 * kStageBytes;    // either two tiles or two halves
+  static constexpr int kStages = 5;
+  static constexpr int kSmem = kQBytes + kStages * kStageBytes + 1024;  // aligned to 1024 inside
+  static constexpr uint32_t kColO = 256;             // S buffers at 0 and 128
 };
 
-// Sequence and first row of query tile `at`; false behind the last one.
-__device__ bool find_tile(const PromptParams& P, int at, int* b_out, int* row_out) {
+struct Work {
+  int q0, nq, k0, nk;  // the sequence's rows and keys
+  int tok0;            // its first token here
+  int head0;           // first of the PACK heads
+  int kvh;
+};
+
+// The CTA's sequence and tokens: tiles of one sequence go from its end to its
+// start, the longest first. False behind the last tile. One warp.
+__device__ bool find_work(const PromptParams& P, int tokens, Work* out) {
   const int lane = threadIdx.x & 31;
+  const int groups = P.hq >> P.pack_log2;
+  const int group = blockIdx.x % groups;
+  int at = blockIdx.x / groups;
   for (int b0 = 0; b0 < P.batch; b0 += 32) {
     const int b = b0 + lane;
-    int n = 0;
-    if (b < P.batch) n = (max(0, P.cu_q[b + 1] - P.cu_q[b]) + kRowsQ - 1) / kRowsQ;
+    int64_t len = 0;
+    if (b < P.batch) len = (int64_t)P.cu_q[b + 1] - P.cu_q[b];
+    if (len < 0 || len > P.total_q) {
+      report_device_error(P.err, FMHA_ERR_INVALID_ARG, kSitePromptLength);
+      len = 0;
+    }
+    const int n = (int)((len + tokens - 1) / tokens);
     int inc = n;
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
@@ -64,8 +115,21 @@ __device__ bool find_tile(const PromptParams& P, int at, int* b_out, int* row_ou
     const unsigned hit = __ballot_sync(kFullMask, at < inc);
     if (hit) {
       const int w = __ffs(hit) - 1;
-      *b_out = b0 + w;
-      *row_out = (at - __shfl_sync(kFullMask, inc - n, w)) * kRowsQ;
+      const int tile = __shfl_sync(kFullMask, inc, w) - 1 - at;  // reversed inside the sequence
+      const int seq = b0 + w;
+      const int64_t q0 = P.cu_q[seq], nq = P.cu_q[seq + 1] - q0;
+      const int64_t k0 = P.cu_kv[seq], nk = P.cu_kv[seq + 1] - k0;
+      if (q0 < 0 || q0 + nq > P.total_q || k0 < 0 || nk < 0 || k0 + nk > P.total_kv) {
+        if (lane == 0) report_device_error(P.err, FMHA_ERR_INVALID_ARG, kSitePromptLength);
+        return false;
+      }
+      out->q0 = (int)q0;
+      out->nq = (int)nq;
+      out->k0 = (int)k0;
+      out->nk = (int)nk;
+      out->tok0 = tile * tokens;
+      out->head0 = group << P.pack_log2;
+      out->kvh = out->head0 / (P.hq / P.hkv);
       return true;
     }
     at -= __shfl_sync(kFullMask, inc, 31);
@@ -73,153 +137,515 @@ __device__ bool find_tile(const PromptParams& P, int at, int* b_out, int* row_ou
   return false;
 }
 
+// Key blocks that tile i of the CTA needs; -1 if it holds no row.
+__device__ __forceinline__ int tile_blocks(const PromptParams& P, const Work& w, int i) {
+  const int tokens = kTileRows >> P.pack_log2;
+  const int first = w.tok0 + i * tokens;
+  if (first >= w.nq) return -1;
+  const int last = min(w.nq, first + tokens) - 1;
+  const int keys = P.causal ? max(0, min(w.nk, last + (w.nk - w.nq) + 1)) : w.nk;
+  return (keys + kKeys - 1) / kKeys;
+}
+
+// One output row on the CUDA cores, by one warp: weights 2^(s*sc + neg) over
+// the row's own `seen` keys, divided by l. For rows that met a NaN or an
+// infinity behind their last key in the tensor cores.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kPromptThreads) prompt_kernel(const __grid_constant__ PromptParams P) {
-  using S = PromptShape<D>;
-  constexpr int kSteps = D / 16;
-  constexpr int kCh = D / 8;
-  extern __shared__ __align__(1024) uint8_t smem[];
-  allow_dependent_launch();
-  grid_dependency_wait();
-  int b, row0;
-  if (!find_tile(P, blockIdx.x, &b, &row0)) return;
-  const int head = blockIdx.y, kvh = head / (P.hq / P.hkv);
-  const int q0 = P.cu_q[b], nq = P.cu_q[b + 1] - q0;
-  const int k0 = P.cu_kv[b], nk = P.cu_kv[b + 1] - k0;
-  if (q0 < 0 || q0 + (int64_t)nq > P.total_q || k0 < 0 || nk < 0 || k0 + (int64_t)nk > P.total_kv) {
-    if (threadIdx.x == 0) report_device_error(P.err, FMHA_ERR_INVALID_ARG, kSitePromptLength);
-    return;
-  }
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int gr = lane >> 2, gc = lane & 3;
-  const uint32_t sq = smem_u32(smem), skv = sq + S::kQ;
-  auto fill = [&](uint32_t dst, const uint16_t* base, int64_t stride, int rows, int have) {
-    for (int e = threadIdx.x; e < rows * kCh; e += kPromptThreads) {
-      const int r = e / kCh, ch = e % kCh;
-      cp_async16(dst + r * S::kRow + ((ch ^ (r & 7)) << 4), base + (r < have ? r : 0) * stride + ch * 8,
-                 r < have ? 16 : 0);
-    }
-  };
-  const int ahead = nk - nq;
-  const int last_row = min(row0 + kRowsQ, nq) - 1;
-  const int keys = P.causal ? max(0, min(nk, last_row + ahead + 1)) : nk;
-  const int tiles = (keys + S::kKeys - 1) / S::kKeys;
-  fill(sq, P.q + (int64_t)(q0 + row0) * P.q_stride + (int64_t)head * D, P.q_stride, kRowsQ, nq - row0);
-  auto load = [&](int t) {
-    if (t < tiles) {
-      const uint32_t at = skv + (t & 1) * 2 * S::kKV;
-      const int64_t r = k0 + (int64_t)t * S::kKeys;
-      fill(at, P.k + r * P.k_stride + (int64_t)kvh * D, P.k_stride, S::kKeys, nk - t * S::kKeys);
-      fill(at + S::kKV, P.v + r * P.v_stride + (int64_t)kvh * D, P.v_stride, S::kKeys,
-           nk - t * S::kKeys);
-    }
-    cp_async_commit();
-  };
-  load(0);
-  float acc[D / 8][4];
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-  const int my0 = row0 + warp * 16 + gr;  // and + 8
-  for (int t = 0; t < tiles; ++t) {
-    load(t + 1);
-    cp_async_wait<1>();
-    __syncthreads();
-    const uint32_t kt = skv + (t & 1) * 2 * S::kKV, vt = kt + S::kKV;
-    float sc[S::kKeys / 8][4] = {};
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      uint32_t a[4];
-      const int ra = warp * 16 + (lane & 15), ca = 2 * s + (lane >> 4);
-      ldsm4(a, sq + ra * S::kRow + ((ca ^ (ra & 7)) << 4));
-#pragma unroll
-      for (int n = 0; n < S::kKeys / 16; ++n) {
-        const int r = n * 16 + (lane & 7) + ((lane >> 4) << 3), ch = 2 * s + ((lane >> 3) & 1);
-        uint32_t w[4];
-        ldsm4(w, kt + r * S::kRow + ((ch ^ (r & 7)) << 4));
-        mma16<BF16>(sc[2 * n], a[0], a[1], a[2], a[3], w[0], w[1]);
-        mma16<BF16>(sc[2 * n + 1], a[0], a[1], a[2], a[3], w[2], w[3]);
+__device__ __noinline__ void row_again(const PromptParams& P, const Work& w, int tok, int head,
+                                       int seen, float neg, float l) {
+  constexpr int kMine = D / 32;  // columns of a lane
+  const int lane = threadIdx.x & 31;
+  const uint16_t* const q = P.q + (int64_t)(w.q0 + tok) * P.q_stride + (int64_t)head * D;
+  const uint16_t* const k = P.k + (int64_t)w.k0 * P.k_stride + (int64_t)w.kvh * D;
+  const uint16_t* const v = P.v + (int64_t)w.k0 * P.v_stride + (int64_t)w.kvh * D + kMine * lane;
+  float o[kMine] = {};
+  for (int j0 = 0; j0 < seen; j0 += 32) {
+    float s = 0.0f;
+    if (j0 + lane < seen) {
+      const uint32_t* const kr = reinterpret_cast<const uint32_t*>(k + (j0 + lane) * P.k_stride);
+      for (int c = 0; c < D / 2; ++c) {
+        const float2 x = unpack2<BF16>(reinterpret_cast<const uint32_t*>(q)[c]);
+        const float2 y = unpack2<BF16>(kr[c]);
+        s = fmaf(x.x, y.x, fmaf(x.y, y.y, s));
       }
     }
-    float down[2];
+    const float p = j0 + lane < seen ? ex2(fmaf(s, P.scale_log2, neg)) : 0.0f;
+    const int have = min(32, seen - j0);
+    for (int j = 0; j < have; ++j) {
+      const float pj = __shfl_sync(kFullMask, p, j);
+      const uint32_t* const vr = reinterpret_cast<const uint32_t*>(v + (j0 + j) * P.v_stride);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int seen = P.causal ? min(nk, my0 + 8 * h + ahead + 1) : nk;  // keys of this row
-      float top = m[h];
-#pragma unroll
-      for (int n = 0; n < S::kKeys / 8; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int key = t * S::kKeys + n * 8 + 2 * gc + j;
-          float& x = sc[n][2 * h + j];
-          x = key < seen ? x * P.scale_log2 : -INFINITY;
-          top = fmaxf(top, x);
-        }
-      top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 2));
-      const float ref = top == -INFINITY ? 0.0f : top;
-      down[h] = exp2f(m[h] - ref);
-      m[h] = top;
-      float sum = 0.0f;
-#pragma unroll
-      for (int n = 0; n < S::kKeys / 8; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float& x = sc[n][2 * h + j];
-          x = exp2f(x - ref);
-          sum += x;
-        }
-      l[h] = l[h] * down[h] + sum;
-    }
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] *= down[j >> 1];
-#pragma unroll
-    for (int n = 0; n < S::kKeys / 16; ++n) {
-      uint32_t hi[4], lo[4];
-      split2<BF16>(sc[2 * n][0], sc[2 * n][1], hi[0], lo[0]);
-      split2<BF16>(sc[2 * n][2], sc[2 * n][3], hi[1], lo[1]);
-      split2<BF16>(sc[2 * n + 1][0], sc[2 * n + 1][1], hi[2], lo[2]);
-      split2<BF16>(sc[2 * n + 1][2], sc[2 * n + 1][3], hi[3], lo[3]);
-#pragma unroll
-      for (int i = 0; i < kCh; i += 2) {
-        const int r = n * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), ch = i + (lane >> 4);
-        uint32_t w[4];
-        ldsm4_trans(w, vt + r * S::kRow + ((ch ^ (r & 7)) << 4));
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          mma16<BF16>(acc[i + j], hi[0], hi[1], hi[2], hi[3], w[2 * j], w[2 * j + 1]);
-          mma16<BF16>(acc[i + j], lo[0], lo[1], lo[2], lo[3], w[2 * j], w[2 * j + 1]);
-        }
+      for (int i = 0; i < kMine / 2; ++i) {
+        const float2 y = unpack2<BF16>(vr[i]);
+        o[2 * i] = fmaf(pj, y.x, o[2 * i]);
+        o[2 * i + 1] = fmaf(pj, y.y, o[2 * i + 1]);
       }
     }
-    __syncthreads();
   }
-  cp_async_wait<0>();
+  uint32_t* const out = reinterpret_cast<uint32_t*>(
+      P.o + (int64_t)(w.q0 + tok) * P.o_stride + (int64_t)head * D + kMine * lane);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    l[h] += __shfl_xor_sync(kFullMask, l[h], 1);
-    l[h] += __shfl_xor_sync(kFullMask, l[h], 2);
-    const int row = my0 + 8 * h;
-    if (row >= nq) continue;
-    const bool none = nk == 0 || (P.causal && row + ahead < 0);
-    const float inv = 1.0f / l[h];
-    uint16_t* const out = P.o + (int64_t)(q0 + row) * P.o_stride + (int64_t)head * D;
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-      const float x = none ? 0.0f : acc[i][2 * h] * inv, y = none ? 0.0f : acc[i][2 * h + 1] * inv;
-      *reinterpret_cast<uint32_t*>(out + 8 * i + 2 * gc) =
-          P.o_bf16 ? pack2<true>(x, y) : pack2<false>(x, y);
-    }
-    if (P.lse && gc == 0)
-      P.lse[(int64_t)(q0 + row) * P.hq + head] = (m[h] + log2f(l[h])) * 0.69314718055994531f;
+  for (int i = 0; i < kMine / 2; ++i) {
+    const float a = o[2 * i] / l, b = o[2 * i + 1] / l;
+    out[i] = P.o_bf16 ? pack2<true>(a, b) : pack2<false>(a, b);
   }
 }
 
+template <int D, bool BF16, bool SPLIT>
+__global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
+    prompt_kernel(const __grid_constant__ PromptParams P) {
+  using S = PromptShape<D>;
+  constexpr int kTiles = S::kTiles, kHalves = S::kHalves, kStages = S::kStages;
+  // Weights in fp16 carry 2^7, so that small ones keep clear of its short exponent.
+  constexpr float kShift = BF16 ? 0.0f : 7.0f;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bars[2 * kStages + 8];
+  __shared__ uint32_t tmem_slot;
+  __shared__ Work work;
+  __shared__ int have_work;
+  __shared__ volatile int abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  allow_dependent_launch();
+  grid_dependency_wait();
+
+  if (warp == 0) {
+    Work w;
+    const bool found = find_work(P, kTiles * (kTileRows >> P.pack_log2), &w);
+    if (lane == 0) {
+      if (found) work = w;
+      have_work = found;
+      abort_flag = 0;
+    }
+  }
+  __syncthreads();
+  if (!have_work) return;
+
+  const uint32_t bar0 = smem_u32(bars);
+  auto bar = [&](int i) { return bar0 + 8 * i; };
+  constexpr int kFull = 0, kEmpty = kStages, kQFull = 2 * kStages, kSFull = kQFull + 1,
+                kPFull = kSFull + 2, kODone = kPFull + 2, kDrain = kODone + 2;
+  if (warp == S::kSoftWarps + 1) {
+    if (lane == 0) {
+      for (int i = 0; i < kStages; ++i) {
+        mbar_init(bar(kFull + i), 1);
+        mbar_init(bar(kEmpty + i), 1);
+      }
+      mbar_init(bar(kQFull), 1);
+      mbar_init(bar(kDrain), 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(bar(kSFull + i), 1);
+        mbar_init(bar(kPFull + i), 4);
+        mbar_init(bar(kODone + i), 1);
+      }
+      fence_mbar_init();
+      fence_async_shared();
+    }
+    __syncwarp();
+    tmem_alloc(smem_u32(&tmem_slot), 512);
+    tmem_fence_before();
+  }
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const Work w = work;
+  const uint32_t sq = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t ring = sq + S::kQBytes;
+  const int n0 = tile_blocks(P, w, 0);
+  const int n1 = kTiles == 2 ? tile_blocks(P, w, 1) : -1;
+  const int blocks = max(n0, n1);
+  auto wait = [&](int b, uint32_t parity) {  // one thread
+    return mbar_wait(bar(b), parity, &abort_flag, P.err, kWaitTimeoutNs, kSitePromptWait);
+  };
+  auto wait_warp = [&](int b, uint32_t parity) {  // a whole warp, of one mind
+    return __all_sync(kFullMask, wait(b, parity)) != 0;
+  };
+
+  if (warp == S::kSoftWarps) {
+    // ---------------------------------------------------------- TMA loads
+    if (lane == 0 && blocks > 0) {
+      const int tokens = kTileRows >> P.pack_log2;
+      mbar_arrive_expect_tx(bar(kQFull), (kTiles == 2 && n1 < 0 ? 1 : 2) * kStageBytes);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (kTiles == 2 && i == 1 && n1 < 0) break;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          tma_load_3d(sq + i * kStageBytes + c * kBlockBytes, &P.map_q,
+                      (kTiles == 2 ? 0 : 128 * i) + 64 * c, w.head0,
+                      w.q0 + w.tok0 + (kTiles == 2 ? i * tokens : 0), bar(kQFull));
+      }
+      int slot = 0, use = 0;  // loads go in the order the MMA warp takes them
+      bool ok = true;
+      auto load = [&](const CUtensorMap* map, int j, int h) {
+        if (!ok) return;
+        if (use > 0 && !wait(kEmpty + slot, (use - 1) & 1)) {
+          ok = false;
+          return;
+        }
+        mbar_arrive_expect_tx(bar(kFull + slot), kStageBytes);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          tma_load_3d(ring + slot * kStageBytes + c * kBlockBytes, map, 128 * h + 64 * c, w.kvh,
+                      w.k0 + j * kKeys, bar(kFull + slot));
+        if (++slot == kStages) {
+          slot = 0;
+          ++use;
+        }
+      };
+      for (int h = 0; h < kHalves; ++h) load(&P.map_k, 0, h);
+      for (int j = 0; j < blocks && ok; ++j) {
+        if (kTiles == 2) {
+          load(&P.map_v, j, 0);
+          if (j + 1 < blocks) load(&P.map_k, j + 1, 0);
+        } else {
+          if (j + 1 < blocks)
+            for (int h = 0; h < kHalves; ++h) load(&P.map_k, j + 1, h);
+          for (int h = 0; h < kHalves; ++h) load(&P.map_v, j, h);
+        }
+      }
+      if (!ok) {
+        // Given up: let this CTA's copies land before its shared memory goes.
+        const uint64_t t0 = globaltimer_ns();
+        for (int i = 0; i < kStages; ++i) {
+          const int uses = use + (i < slot ? 1 : 0);
+          if (uses == 0) continue;
+          while (!mbar_try_wait(bar(kFull + i), (uses - 1) & 1) &&
+                 globaltimer_ns() - t0 < kStallTimeoutNs) {
+          }
+        }
+      }
+    }
+  } else if (warp == S::kSoftWarps + 1) {
+    // ---------------------------------------------------------- MMAs
+    constexpr uint32_t kIdQK = umma_idesc(BF16, 128, false);
+    constexpr uint32_t kIdPV = umma_idesc(BF16, 128, true);
+    bool ok = blocks > 0 && wait_warp(kQFull, 0);
+    int slot = 0, use = 0;
+    auto take = [&]() {  // waits for the next stage; its address
+      ok = ok && wait_warp(kFull + slot, use & 1);
+      return ring + slot * kStageBytes;
+    };
+    auto done = [&]() {  // frees it once the MMAs issued so far are through
+      if (lane == 0) umma_commit(bar(kEmpty + slot));
+      if (++slot == kStages) {
+        slot = 0;
+        ++use;
+      }
+    };
+    // S = Q K^T over one 128-column part.
+    auto qk = [&](uint32_t s_col, uint32_t q, uint32_t k, bool first) {
+      if (lane != 0) return;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t off = (i >> 2) * kBlockBytes + (i & 3) * 32;
+        umma_ss(tmem + s_col, umma_desc(q + off, 16, 1024), umma_desc(k + off, 16, 1024), kIdQK,
+                !(first && i == 0));
+      }
+    };
+    // O += P V over one 128-column part.
+    auto pv = [&](uint32_t o_col, uint32_t p_col, uint32_t v, bool first) {
+      if (lane != 0) return;
+#pragma unroll
+      for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          umma_ts(tmem + o_col, tmem + p_col + part * 64 + i * 8,
+                  umma_desc(v + i * 2048, kBlockBytes, 1024), kIdPV, !(first && part == 0 && i == 0));
+    };
+    // V rows behind the sequence's end, if any, become zeros.
+    auto trim = [&](uint32_t v, int j) {
+      const int have = w.nk - j * kKeys;
+      if (have >= kKeys) return;
+      for (int e = lane; e < (kKeys - have) * 16; e += 32) {
+        const uint32_t at = v + (e & 1) * kBlockBytes + (have + (e >> 4)) * 128 + ((e >> 1) & 7) * 16;
+        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
+      }
+      fence_async_shared();
+      __syncwarp();
+    };
+    if constexpr (kTiles == 2) {
+      if (ok) {
+        const uint32_t k = take();
+        if (ok) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if ((i ? n1 : n0) > 0) {
+              qk(128 * i, sq + i * kStageBytes, k, true);
+              if (lane == 0) umma_commit(bar(kSFull + i));
+            }
+          done();
+        }
+      }
+      for (int j = 0; j < blocks && ok; ++j) {
+        const uint32_t v = take();
+        if (!ok) break;
+        const int v_slot = slot;
+        if (++slot == kStages) {
+          slot = 0;
+          ++use;
+        }
+        trim(v, j);
+        uint32_t k = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int n = i ? n1 : n0;
+          if (j < n) {
+            ok = ok && wait_warp(kPFull + i, j & 1);
+            if (!ok) break;
+            tmem_fence_after();
+            pv(S::kColO + 128 * i, 128 * i, v, j == 0);
+            if (lane == 0 && j + 1 == n) umma_commit(bar(kODone + i));
+          }
+          if (i == 1 && lane == 0) umma_commit(bar(kEmpty + v_slot));
+          if (j + 1 < n) {
+            if (k == 0) k = take();
+            if (!ok) break;
+            qk(128 * i, sq + i * kStageBytes, k, true);
+            if (lane == 0) umma_commit(bar(kSFull + i));
+          }
+        }
+        if (ok && j + 1 < blocks) done();
+      }
+    } else {
+      auto scores = [&](int j) {
+        for (int h = 0; h < kHalves && ok; ++h) {
+          const uint32_t k = take();
+          if (!ok) return;
+          qk(128 * (j & 1), sq + h * kStageBytes, k, h == 0);
+          done();
+        }
+        if (lane == 0 && ok) umma_commit(bar(kSFull + (j & 1)));
+      };
+      if (ok) scores(0);
+      for (int j = 0; j < blocks && ok; ++j) {
+        if (j + 1 < blocks) scores(j + 1);
+        ok = ok && wait_warp(kPFull + (j & 1), (j >> 1) & 1);
+        if (!ok) break;
+        tmem_fence_after();
+        for (int h = 0; h < kHalves && ok; ++h) {
+          const uint32_t v = take();
+          if (!ok) break;
+          trim(v, j);
+          pv(S::kColO + 128 * h, 128 * (j & 1), v, j == 0);
+          done();
+        }
+        if (lane == 0 && ok) umma_commit(bar(kODone));
+      }
+    }
+    if (blocks > 0 && !ok && lane == 0) {
+      // Given up: let the MMAs in flight end before their memory goes.
+      umma_commit(bar(kDrain));
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(bar(kDrain), 0) && globaltimer_ns() - t0 < kStallTimeoutNs) {
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------- softmax
+    const int tile = warp >> 2;
+    const int row = threadIdx.x & 127;
+    const uint32_t lanes = tmem + ((uint32_t)(row & ~31) << 16);
+    const int n = tile ? n1 : n0;
+    const int tokens = kTileRows >> P.pack_log2;
+    const int tok_base = w.tok0 + tile * tokens;
+    const int tok = tok_base + (row >> P.pack_log2);
+    const int ahead = w.nk - w.nq;
+    const int seen = P.causal ? max(0, min(w.nk, tok + ahead + 1)) : w.nk;  // keys of this row
+    const int warp_tok = tok_base + ((row & ~31) >> P.pack_log2);
+    const int least = P.causal ? min(w.nk, warp_tok + ahead + 1) : w.nk;  // of the warp's first row
+    const float sc = P.scale_log2;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      const int buf = kTiles == 2 ? tile : j & 1;
+      ok = wait_warp(kSFull + buf, kTiles == 2 ? j & 1 : (j >> 1) & 1);
+      if (!ok) break;
+      tmem_fence_after();
+      const uint32_t s_at = lanes + 128 * buf;
+      uint32_t x[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(x[c], s_at + 32 * c);
+      tmem_wait_ld();
+      if ((j + 1) * kKeys > least) {
+        const int left = seen - j * kKeys;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (32 * c + i >= left) x[c][i] = 0xff800000u;
+      }
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], __uint_as_float(x[c][i]));
+      const float now = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+      if (j == 0) {
+        m = now;
+      } else {
+        const bool rise = (now - m) * sc > kSlack;
+        if (__any_sync(kFullMask, rise)) {
+          // The scores of block j follow P.V of block j-1 (head_dim 128), or of j-2 (256).
+          if (kTiles == 1) {
+            ok = wait_warp(kODone, (j - 1) & 1);
+            if (!ok) break;
+            tmem_fence_after();
+          }
+          float f = 1.0f;
+          if (rise) {
+            f = ex2((m - now) * sc);
+            m = now;
+            l *= f;
+          }
+          __syncwarp();
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            const uint32_t at = lanes + S::kColO + (kTiles == 2 ? 128 * tile : 0) + 32 * c;
+            uint32_t y[32];
+            tmem_ld32(y, at);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+            tmem_st32(at, y);
+          }
+        }
+      }
+      const float neg = m == -INFINITY ? 0.0f : kShift - m * sc;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float p = ex2(fmaf(__uint_as_float(x[c][i]), sc, neg));
+          sum[i & 3] += p;
+          x[c][i] = __float_as_uint(p);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t hi[32], lo[SPLIT ? 32 : 1];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float a = __uint_as_float(x[2 * c + (i >> 4)][(2 * i) & 31]);
+          const float b = __uint_as_float(x[2 * c + (i >> 4)][((2 * i) & 31) + 1]);
+          if constexpr (SPLIT)
+            split2<BF16>(a, b, hi[i], lo[i]);
+          else
+            hi[i] = pack2<BF16>(a, b);
+        }
+        tmem_st32(s_at + 32 * c, hi);
+        if constexpr (SPLIT) tmem_st32(s_at + 64 + 32 * c, lo);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_wait_st();
+      tmem_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kPFull + buf));
+    }
+
+    if (ok && n > 0) {
+      if (kTiles == 2) {
+        ok = wait_warp(kODone + tile, 0);
+      } else {
+        // One phase after the other: the last but one may still be open.
+        if (n > 1) ok = wait_warp(kODone, n & 1);
+        ok = ok && wait_warp(kODone, (n - 1) & 1);
+      }
+      tmem_fence_after();
+    }
+    if (ok && n >= 0) {
+      const bool mine = tok < w.nq;
+      const int head = w.head0 + (row & ((1 << P.pack_log2) - 1));
+      const bool none = seen == 0;
+      const float inv = 1.0f / l;
+      uint16_t* const out = P.o + (int64_t)(w.q0 + tok) * P.o_stride + (int64_t)head * D;
+      bool nan = false;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t y[32];
+        if (n > 0) {
+          tmem_ld32(y, lanes + S::kColO + (kTiles == 2 ? 128 * tile : 0) + 32 * c);
+          tmem_wait_ld();
+        }
+        if (mine) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t z[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float a = none ? 0.0f : __uint_as_float(y[8 * i + 2 * e]) * inv;
+              const float b = none ? 0.0f : __uint_as_float(y[8 * i + 2 * e + 1]) * inv;
+              nan |= isnan(a) || isnan(b);
+              z[e] = P.o_bf16 ? pack2<true>(a, b) : pack2<false>(a, b);
+            }
+            *reinterpret_cast<uint4*>(out + 32 * c + 8 * i) = make_uint4(z[0], z[1], z[2], z[3]);
+          }
+        }
+        __syncwarp();
+      }
+      if (mine && P.lse)
+        P.lse[(int64_t)(w.q0 + tok) * P.hq + head] =
+            none ? -INFINITY : (m * sc + (log2f(l) - kShift)) * 0.69314718055994531f;
+      // NaN in rows whose weights are sound (l = 0: every score -inf, 0/0).
+      unsigned again = __ballot_sync(kFullMask, nan && l > 0.0f && l <= FLT_MAX);
+      const float neg = m == -INFINITY ? 0.0f : kShift - m * sc;
+      while (again) {
+        const int r = __ffs(again) - 1;
+        again &= again - 1;
+        row_again<D, BF16>(P, w, __shfl_sync(kFullMask, tok, r), __shfl_sync(kFullMask, head, r),
+                           __shfl_sync(kFullMask, seen, r), __shfl_sync(kFullMask, neg, r),
+                           __shfl_sync(kFullMask, l, r));
+      }
+    }
+    tmem_fence_before();
+  }
+  __syncthreads();
+  if (warp == S::kSoftWarps + 1) tmem_free(tmem, 512);
+}
+
 using PromptFn = void (*)(const PromptParams);
+
+template <int D>
+PromptFn prompt_fn(bool bf16, bool split) {
+  if (!bf16) return prompt_kernel<D, false, false>;
+  return split ? prompt_kernel<D, true, true> : prompt_kernel<D, true, false>;
+}
+
+// The driver's tensor-map encoder, looked up once.
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                              const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encoder() {
+  static const EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) !=
+            cudaSuccess ||
+        found != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      return EncodeFn(nullptr);
+    }
+    return reinterpret_cast<EncodeFn>(p);
+  }();
+  return fn;
+}
+
+// [rows, heads, d] of 16-bit elements, in boxes of `rows_box` x `heads_box` x 64 columns.
+bool encode(CUtensorMap* map, bool bf16, const void* p, int d, int heads, int rows, int64_t stride,
+            int heads_box, int rows_box) {
+  const EncodeFn fn = encoder();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)stride * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)heads_box, (cuuint32_t)rows_box};
+  const cuuint32_t ones[3] = {1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+            const_cast<void*>(p), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 }  // namespace
 }  // namespace fmha
@@ -278,13 +704,26 @@ extern "C" fmha_status_t fmha_prompt(const void* Q, const void* K, const void* V
   P.o_bf16 = o_dtype == FMHA_DTYPE_BF16;
   P.err = dev.err;
   const bool bf16 = dtype == FMHA_DTYPE_BF16;
-  const PromptFn fn = head_dim == 128 ? (bf16 ? prompt_kernel<128, true> : prompt_kernel<128, false>)
-                                      : (bf16 ? prompt_kernel<256, true> : prompt_kernel<256, false>);
+  const int g = num_heads_q / num_heads_kv;
+  while (P.pack_log2 < 7 && (g >> P.pack_log2) % 2 == 0) ++P.pack_log2;
+  const int pack = 1 << P.pack_log2;
+  // Without keys no map is used; K's then describes Q.
+  const bool keys = total_kv > 0;
+  if (!encode(&P.map_q, bf16, Q, head_dim, num_heads_q, total_q, q_stride, pack, kTileRows / pack) ||
+      !encode(&P.map_k, bf16, keys ? K : Q, head_dim, keys ? num_heads_kv : num_heads_q,
+              keys ? total_kv : total_q, keys ? k_stride : q_stride, 1, kKeys) ||
+      !encode(&P.map_v, bf16, keys ? V : Q, head_dim, keys ? num_heads_kv : num_heads_q,
+              keys ? total_kv : total_q, keys ? v_stride : q_stride, 1, kKeys))
+    return FMHA_ERR_CUDA;
+  const bool split = bf16 && !P.o_bf16;
+  const PromptFn fn = head_dim == 128 ? prompt_fn<128>(bf16, split) : prompt_fn<256>(bf16, split);
   const int smem = head_dim == 128 ? PromptShape<128>::kSmem : PromptShape<256>::kSmem;
+  const int threads = head_dim == 128 ? PromptShape<128>::kThreads : PromptShape<256>::kThreads;
   if ((st = ensure_smem(reinterpret_cast<const void*>(fn), smem)) != FMHA_OK) return st;
-  // No more tiles than this, whatever the lengths: each sequence has one that is not full.
-  const int64_t tiles = (int64_t)batch + total_q / kRowsQ;
-  if (tiles > 0x7fffffff) return FMHA_ERR_UNSUPPORTED;
-  return launch_serving(fn, dim3((unsigned)tiles, num_heads_q), kPromptThreads, smem,
+  // No more work than this, whatever the lengths: each sequence has one part that is not full.
+  const int tokens = (head_dim == 128 ? 2 : 1) * kTileRows / pack;
+  const int64_t parts = ((int64_t)batch + total_q / tokens) * (num_heads_q / pack);
+  if (parts > 0x7fffffff) return FMHA_ERR_UNSUPPORTED;
+  return launch_serving(fn, dim3((unsigned)parts), threads, smem,
                         reinterpret_cast<cudaStream_t>(stream), P);
 }

@@ -532,6 +532,28 @@ def test_prompt_strided_rows(cuda):
     assert bool((wide[:, :hq] == 7.0).all())
 
 
+@pytest.mark.parametrize("d", [128, 256])
+def test_prompt_nonfinite(cuda, d):
+    """NaN and infinities reach the rows that see their token, and only those."""
+    g = gen(23)
+    n, hq, hkv = 200, 2, 1
+    q, k, v = randn((n, hq, d), g, BF16), randn((n, hkv, d), g, BF16), randn((n, hkv, d), g, BF16)
+    k[150, 0, 3] = float("nan")
+    v[100, 0, 7] = float("inf")
+    v[120, 0, 9] = float("nan")
+    q[20, 1] = float("nan")
+    o = fmha_b200.fmha_prompt(q, k, v, starts([n]))
+    torch.cuda.synchronize()
+    nan = torch.zeros_like(o, dtype=torch.bool)
+    nan[150:] = True
+    nan[120:, :, 9] = True
+    nan[20, 1] = True
+    assert torch.equal(torch.isnan(o), nan)
+    inf = torch.zeros_like(nan)
+    inf[100:150, :, 7] = True
+    assert torch.equal(torch.isinf(o), inf)
+
+
 def test_prompt_leaves_out_what_is_impossible(cuda):
     g = gen(24)
     hq, hkv, d = 4, 2, 128
