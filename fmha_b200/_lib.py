@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "libfmha_b200.so")
@@ -21,7 +22,6 @@ VARIANT_AUTO, VARIANT_BULK, VARIANT_LDG = 0, 1, 2
 DTYPE_BF16, DTYPE_FP16, DTYPE_E4M3 = 0, 1, 2
 VARIANTS = {"auto": VARIANT_AUTO, "bulk": VARIANT_BULK, "ldg": VARIANT_LDG}
 
-# Every symbol include/fmha.h declares, with (restype, argtypes).
 _vp, _i, _i64, _u64, _u32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_uint64, ctypes.c_uint32
 _f = ctypes.c_float
 
@@ -30,11 +30,51 @@ class PagedCacheStruct(ctypes.Structure):
     """fmha_paged_cache_t (include/fmha.h)."""
     _fields_ = [("k", _vp), ("v", _vp), ("block_table", _vp), ("seqlens_kv", _vp),
                 ("page_stride", _i64), ("head_stride", _i64), ("token_stride", _i64),
-                ("table_stride", _i64), ("num_pages", ctypes.c_int32),
-                ("page_size", ctypes.c_int32), ("max_pages", ctypes.c_int32),
-                ("dtype", ctypes.c_int32), ("k_scale", _f), ("v_scale", _f)]
+                ("table_stride", _i64), ("num_pages", _i), ("page_size", _i), ("max_pages", _i),
+                ("dtype", _i), ("k_scale", _f), ("v_scale", _f)]
 
 
+class RopeAppendArgs(ctypes.Structure):
+    """fmha_rope_append_args_t."""
+    _fields_ = [(n, _vp) for n in ("q", "k", "v", "q_out", "k_out", "cu_seqlens_q", "cos_table",
+                                   "sin_table")] + \
+               [(n, _i64) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride",
+                                    "k_out_stride")] + [("cache", PagedCacheStruct)] + \
+               [(n, _i) for n in ("total_tokens", "batch", "num_heads_q", "num_heads_kv",
+                                  "head_dim", "rotary_dim", "max_position", "interleaved", "dtype")]
+
+
+class PagedDecodeArgs(ctypes.Structure):
+    """fmha_paged_decode_args_t."""
+    _fields_ = [(n, _vp) for n in ("q", "o", "lse", "workspace")] + \
+               [(n, _i64) for n in ("workspace_bytes", "q_stride", "o_stride")] + \
+               [("cache", PagedCacheStruct)] + \
+               [(n, _i) for n in ("batch", "num_heads_q", "num_heads_kv", "head_dim", "dtype",
+                                  "o_dtype")] + [("softmax_scale", _f)]
+
+
+class PromptArgs(ctypes.Structure):
+    """fmha_prompt_args_t."""
+    _fields_ = [(n, _vp) for n in ("q", "k", "v", "o", "lse", "cu_seqlens_q", "cu_seqlens_kv")] + \
+               [(n, _i64) for n in ("q_stride", "k_stride", "v_stride", "o_stride")] + \
+               [(n, _i) for n in ("total_q", "total_kv", "batch", "num_heads_q", "num_heads_kv",
+                                  "head_dim", "causal", "dtype", "o_dtype")] + \
+               [("softmax_scale", _f)]
+
+
+def packer(cls):
+    """The bytes of an argument struct from its values in order (nested structs' values in
+    place), several times faster than filling the ctypes object."""
+    codes = {_vp: "P", _i64: "q", _i: "i", _f: "f"}
+
+    def walk(c):
+        return "".join(walk(t) if issubclass(t, ctypes.Structure) else codes[t] for _, t in c._fields_)
+    s = struct.Struct("@" + walk(cls) + "0q")
+    assert s.size == ctypes.sizeof(cls)
+    return s.pack
+
+
+# Every symbol include/fmha.h declares, with (restype, argtypes).
 SIGNATURES = {
     "fmha_forward": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "fmha_forward_variant": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
@@ -43,13 +83,10 @@ SIGNATURES = {
     "fmha_forward_varlen_variant": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i,
                                          ctypes.c_float, _i, _vp]),
     "fmha_forward_append": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
-    "fmha_rope_append": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i,
-                              _i64, _i64, _i64, _i64, _i64, _i, _i, _i, _i, _vp]),
-    "fmha_paged_decode_workspace": (_i64, [_i, _i, _i]),
-    "fmha_paged_decode": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i64, _i64, _f, _i, _i, _vp,
-                               _i64, _vp]),
-    "fmha_prompt": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i64, _i64,
-                         _i64, _i64, _f, _i, _i, _i, _vp]),
+    "fmha_rope_append": (_i, [_vp, _vp]),
+    "fmha_paged_decode_workspace": (_i64, [_i, _i, _i, _i64]),
+    "fmha_paged_decode": (_i, [_vp, _vp]),
+    "fmha_prompt": (_i, [_vp, _vp]),
     "fmha_status_string": (ctypes.c_char_p, [_i]),
     "fmha_device_error": (_i, [ctypes.POINTER(_i)]),
     "fmha_fill_normal_bf16": (_i, [_vp, _i64, _u64, _u32, _i64, _vp]),

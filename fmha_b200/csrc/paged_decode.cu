@@ -21,21 +21,26 @@
 // by a power of two that puts its largest element just below 2^15.
 //
 // Split. A unit is one (sequence, kv head, up to 16 of its query heads); a
-// tile is 16 of its tokens. All tiles of all units, one after the other, are
-// dealt out to the CTAs in equal contiguous ranges whatever the lengths, so
-// ragged batches and a single long sequence fill the card alike. Each CTA
-// finds its range from a prefix sum over the lengths, which are only known on
-// the device; a captured launch therefore stays right as sequences grow. A
-// unit that crosses from one CTA into the next leaves partial results in the
-// workspace (at most two per CTA), which a second small kernel joins. When
-// the block table says that no unit can be longer than kWholeTiles tiles, CTAs
-// take whole units and nothing is left to join.
+// tile is 16 of its tokens (32 of an e4m3 cache). All tiles of all units, one
+// after the other, are dealt out in equal contiguous ranges to the CTAs and
+// within them to the warps, whatever the lengths, so ragged batches and a
+// single long sequence fill the card alike. A unit counts one tile more than
+// it has, for its query's load and its output. Each CTA finds its ranges from
+// a prefix sum over the lengths, which are only known on the device; a
+// captured launch therefore stays right as sequences grow. A warp writes the
+// outputs of units that begin and end in its range; the at most two others
+// wait in shared memory until the CTA's warps are done and are joined there.
+// A unit that crosses from one CTA into the next leaves a partial result in
+// the workspace (at most two per CTA), which a second small kernel joins.
+// When the block table says that no unit can be longer than kWholeTokens,
+// CTAs take whole units and nothing is left to join.
 //
-// Inside a CTA the warps take tiles in turn. Each has its own ring of tiles
-// in shared memory, filled by its own 16-byte cp.async (zero-filled behind
-// the sequence's end, so that what lies in unused rows, NaN included, never
-// meets the MMA), running on into the next unit while the current one is
-// joined across the warps.
+// Each warp has its own ring of tiles in shared memory, filled by its own
+// 16-byte cp.async (zero-filled behind the sequence's end, so that what lies
+// in unused rows, NaN included, never meets the MMA), running on into the
+// next unit while the current one ends. Warps wait for one another only at
+// the end: joining every unit across the CTA's warps instead cost 1 to 2 us a
+// unit, and 230 us instead of 146 us on 131 sequences of 16 to 8192 tokens.
 #include <cuda_runtime.h>
 
 #include <cfloat>
@@ -46,14 +51,14 @@
 #include "decode_common.cuh"
 #include "serving.hpp"
 #include "serving_mma.cuh"
+#include "tcgen05.cuh"
 
 namespace fmha {
 namespace {
 
-constexpr int kTile = 16;          // tokens
 constexpr int kMaxCtas = 160;      // parts the work is dealt into, at most
 constexpr int kMaxRows = 16;       // query heads of a unit
-constexpr int kWholeTiles = 32;    // units up to this length are not split
+constexpr int kWholeTokens = 512;  // units up to this length are not split
 constexpr int kJoinThreads = 256;  // of the joining kernel
 
 struct DecodeParams {
@@ -68,6 +73,8 @@ struct DecodeParams {
   int chunks;  // units per (sequence, kv head)
   int64_t q_stride, o_stride;
   float scale_log2;  // log2(e) * softmax_scale * k_scale
+  uint32_t page_mul;  // token / page_size = token * page_mul >> page_shift, tokens below 2^31
+  int page_shift;
   int whole;         // CTAs take whole units
   int o_bf16;
   float shift;        // weight_shift of the kernel
@@ -77,93 +84,27 @@ struct DecodeParams {
   unsigned int* err;
 };
 
-// ------------------------------------------------------------ the work list
+// ------------------------------------------------------------ shapes
 
-struct Place {  // a tile of a unit
-  int b;        // sequence
-  int hu;       // (kv head, chunk) of the sequence
-  int tile;
-};
-
-__device__ __forceinline__ int tiles_of(const DecodeParams& P, int b) {
-  const int n = P.cache.seqlens_kv[b];
-  const int64_t most = (int64_t)P.cache.max_pages * P.cache.page_size;
-  if (n < 0 || n > most) return 1;  // impossible: left out, and reported where it is met
-  return n == 0 ? 1 : (n + kTile - 1) / kTile;  // an empty one still writes its zeros
-}
-
-// With the whole CTA: thread i takes a contiguous run of sequences, scan[i]
-// becomes the tiles (of one unit each) before its run, and their total is
-// returned.
-template <int THREADS>
-__device__ int64_t scan_lengths(const DecodeParams& P, int64_t* scan) {
-  const int per = (P.batch + THREADS - 1) / THREADS;
-  const int b0 = min(P.batch, (int)threadIdx.x * per), b1 = min(P.batch, b0 + per);
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += tiles_of(P, b);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t inc = mine;
-#pragma unroll
-  for (int s = 1; s < 32; s <<= 1) {
-    const int64_t y = __shfl_up_sync(kFullMask, inc, s);
-    if (lane >= s) inc += y;
-  }
-  __shared__ int64_t warp_sum[THREADS / 32];
-  if (lane == 31) warp_sum[warp] = inc;
-  __syncthreads();
-  int64_t before = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) before += warp_sum[w];
-    total += warp_sum[w];
-  }
-  scan[threadIdx.x] = before + inc - mine;
-  __syncthreads();
-  return total;
-}
-
-// The thread whose run holds tile number `at` of the list of all tiles writes
-// its place; a number past the list's end is the place behind it.
-template <int THREADS>
-__device__ void locate(const DecodeParams& P, const int64_t* scan, int64_t at, int64_t total,
-                       Place* out) {
-  const int hu = P.hkv * P.chunks;
-  if (at >= total * hu) {
-    if (threadIdx.x == 0) *out = {P.batch, 0, 0};
-    return;
-  }
-  const int per = (P.batch + THREADS - 1) / THREADS;
-  const int b0 = min(P.batch, (int)threadIdx.x * per), b1 = min(P.batch, b0 + per);
-  int64_t base = scan[threadIdx.x] * hu;
-  const int64_t next = (threadIdx.x + 1 < THREADS ? scan[threadIdx.x + 1] : total) * hu;
-  if (at < base || at >= next) return;
-  for (int b = b0; b < b1; ++b) {
-    const int n = tiles_of(P, b);
-    if (at < base + (int64_t)n * hu) {
-      const int64_t r = at - base;
-      *out = {b, (int)(r / n), (int)(r % n)};
-      return;
-    }
-    base += (int64_t)n * hu;
-  }
-}
-
-// ------------------------------------------------------------ the kernel
-
-template <int D, bool F8>
+template <int D, bool F8, bool WIDE>
 struct DecodeShape {
   static constexpr int kElem = F8 ? 1 : 2;
   static constexpr int kRowBytes = D * kElem;
-  static constexpr int kChunks = kRowBytes / 16;       // 16-byte pieces of a row
-  static constexpr int kHalf = kTile * kRowBytes;      // K or V of a tile
+  static constexpr int kChunks = kRowBytes / 16;  // 16-byte pieces of a row
+  static constexpr int kSub = F8 && !(WIDE && D == 256) ? 2 : 1;  // 16-token steps of a tile
+  static constexpr int kTile = 16 * kSub;
+  static constexpr int kRows = WIDE ? 16 : 8;
+  static constexpr int kHalf = kTile * kRowBytes;  // K or V of a tile
   static constexpr int kStage = 2 * kHalf;
-  static constexpr int kWarps = D == 128 ? 8 : F8 ? 6 : 4;
+  static constexpr int kWarps = D == 128 ? (WIDE ? 6 : 8) : (F8 && WIDE ? 5 : 4);
   static constexpr int kThreads = 32 * kWarps;
-  static constexpr int kStages = D == 128 && F8 ? 6 : 3;
+  static constexpr int kStages = D == 256 && WIDE && !F8 ? 2 : 3;
   static constexpr int kPad = D + 4;  // floats of a row of partial results
-  static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr int kJoinO = kWarps * 8 * kPad * 4;
-  static constexpr int kSmem = kRing + kJoinO;
+  static constexpr int kRing = kStages * kStage;  // of a warp
+  static constexpr int kHold = kRows * kPad * 4;  // a warp's partial result of its first unit
+  static constexpr int kSmem = kWarps * (kRing + kHold);
+  static_assert(2 * kWarps <= 16, "a lane of a half-warp for each held result");
+  static_assert(kHold <= kRing, "the last unit's partial result goes where the ring was");
   static_assert(kSmem <= 230400, "2 KB of a CTA's 227 KB are left to static arrays");
 };
 
@@ -173,121 +114,212 @@ __host__ __device__ constexpr float weight_shift() {
   return BF16 && !F8 ? 0.0f : 15.0f;
 }
 
-// Element offset of a token's row in the pages, or -1 where there is none.
-__device__ __forceinline__ int64_t token_offset(const DecodeParams& P, int b, int token, int len) {
-  if (token >= len) return -1;
-  const int in_table = token / P.cache.page_size;
-  const int page = P.cache.block_table[b * P.cache.table_stride + in_table];
-  if (page < 0 || page >= P.cache.num_pages) {
-    report_device_error(P.err, FMHA_ERR_INVALID_ARG, kSiteDecodePage);
-    return -1;
-  }
-  return page * P.cache.page_stride +
-         (int64_t)(token - in_table * P.cache.page_size) * P.cache.token_stride;
+// ------------------------------------------------------------ the work list
+
+struct Place {  // a tile of a unit; units are numbered sequence by sequence
+  int unit;
+  int tile;
+};
+
+template <int TILE>
+__device__ __forceinline__ int tiles_of(const DecodeParams& P, int b) {
+  const int n = P.cache.seqlens_kv[b];
+  const int64_t most = (int64_t)P.cache.max_pages * P.cache.page_size;
+  if (n <= 0 || n > most) return 1;  // an empty one writes its zeros, an impossible one is reported
+  return (n - 1) / TILE + 1;
 }
 
+// The list of the units [u0, u1): a unit of n tiles takes n + 1 positions.
+// Thread i of the CTA sums a contiguous run of their sequences; before[i]
+// becomes the positions in front of its run.
+template <int TILE, int THREADS>
+struct WorkList {
+  const DecodeParams& P;
+  int hu, u0, u1;
+  int64_t* before;
+  int b_lo, per;  // first sequence, sequences of a run
+
+  __device__ int first(int b) const { return max(u0, b * hu); }
+  __device__ int64_t span(int b, int n) const {
+    return (int64_t)(min(u1, (b + 1) * hu) - first(b)) * (n + 1);
+  }
+  __device__ int64_t sum(int64_t* warp_sum) {  // all positions
+    b_lo = u0 / hu;
+    const int n = u1 > u0 ? (u1 - 1) / hu + 1 - b_lo : 0;
+    per = (n + THREADS - 1) / THREADS;
+    const int b0 = min(n, (int)threadIdx.x * per), b1 = min(n, b0 + per);
+    int64_t mine = 0;
+    for (int b = b_lo + b0; b < b_lo + b1; ++b) mine += span(b, tiles_of<TILE>(P, b));
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t inc = mine;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const int64_t y = __shfl_up_sync(kFullMask, inc, s);
+      if (lane >= s) inc += y;
+    }
+    if (lane == 31) warp_sum[warp] = inc;
+    __syncthreads();
+    int64_t ahead = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) ahead += warp_sum[w];
+      total += warp_sum[w];
+    }
+    before[threadIdx.x] = ahead + inc - mine;
+    __syncthreads();
+    return total;
+  }
+  // The place of position `at`; any thread, after sum().
+  __device__ Place locate(int64_t at, int64_t total) const {
+    if (at >= total) return {u1, 0};
+    int l = 0, r = THREADS;  // before[l] <= at < before[r], the last such run
+    while (r - l > 1) {
+      const int m = (l + r) >> 1;
+      if (before[m] <= at) l = m; else r = m;
+    }
+    int64_t base = before[l];
+    for (int b = b_lo + l * per;; ++b) {
+      const int n = tiles_of<TILE>(P, b);
+      const int64_t here = span(b, n);
+      if (at < base + here) {
+        const int64_t in = at - base;
+        const int u = here <= 0x7fffffff ? (int)((uint32_t)in / (uint32_t)(n + 1)) : (int)(in / (n + 1));
+        const int tile = (int)(in - (int64_t)u * (n + 1));
+        return tile == n ? Place{first(b) + u + 1, 0} : Place{first(b) + u, tile};
+      }
+      base += here;
+    }
+  }
+};
+
+// ------------------------------------------------------------ the kernel
+
 template <int D, bool BF16, bool F8, bool WIDE>
-__global__ void __launch_bounds__((DecodeShape<D, F8>::kThreads), 1)
+__global__ void __launch_bounds__((DecodeShape<D, F8, WIDE>::kThreads), 1)
     paged_decode_kernel(const __grid_constant__ DecodeParams P) {
-  using S = DecodeShape<D, F8>;
+  using S = DecodeShape<D, F8, WIDE>;
   constexpr bool kB = BF16 && !F8;  // type of the MMA's operands: e4m3 goes through fp16
   constexpr int kSteps = D / 16;    // MMA steps along head_dim
+  constexpr int kW = S::kWarps, kH = WIDE ? 2 : 1;
   constexpr float kShift = weight_shift<BF16, F8>();
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ Place range[2];
-  __shared__ float2 join_ml[S::kWarps][kMaxRows];
-  __shared__ uint32_t tile_mask[S::kWarps][S::kStages];
+  __shared__ Place range[kW + 1];
+  __shared__ int64_t warp_sum[kW];
+  __shared__ int slot_unit[2 * kW];  // units left for joining: warp w's first and last
+  __shared__ int slot_ends[2 * kW];   // whether the unit ends there
+  __shared__ float2 slot_ml[2 * kW][S::kRows];
+  __shared__ uint32_t tile_mask[kW][S::kStages];
   allow_dependent_launch();
   grid_dependency_wait();
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int gr = lane >> 2, gc = lane & 3;
   const int HU = P.hkv * P.chunks;
-  int64_t per = 0;  // tiles of a CTA
+  if (threadIdx.x < 2 * kW) slot_unit[threadIdx.x] = -1;
 
-  // This CTA's range of tiles, [range[0], range[1]).
-  if (P.whole) {
-    if (threadIdx.x < 2) {
-      const int64_t u = (int64_t)P.batch * HU * (blockIdx.x + threadIdx.x) / gridDim.x;
-      range[threadIdx.x] = {(int)(u / HU), (int)(u % HU), 0};
+  // The CTA's positions [lo, hi) of the list, and its warps' places there.
+  int64_t per = 0, hi_at;
+  {
+    const int units = P.batch * HU;
+    const int u0 = P.whole ? (int)((int64_t)units * blockIdx.x / gridDim.x) : 0;
+    const int u1 = P.whole ? (int)((int64_t)units * (blockIdx.x + 1) / gridDim.x) : units;
+    WorkList<S::kTile, S::kThreads> list{P, HU, u0, u1,
+                                         reinterpret_cast<int64_t*>(smem), 0, 0};  // no ring yet
+    const int64_t total = list.sum(warp_sum);
+    int64_t lo = 0;
+    hi_at = total;
+    if (!P.whole) {
+      per = total <= 0x7fffffff ? (int64_t)(((uint32_t)total + gridDim.x - 1) / gridDim.x)
+                                : (total + gridDim.x - 1) / gridDim.x;
+      if (per < kW) per = kW;
+      lo = min(total, per * blockIdx.x);
+      hi_at = min(total, lo + per);
+      if (threadIdx.x == 0) P.part_unit[blockIdx.x] = make_int2(-1, 0);
     }
-  } else {
-    int64_t* const scan = reinterpret_cast<int64_t*>(smem);  // before the ring is in use
-    const int64_t total = scan_lengths<S::kThreads>(P, scan);
-    per = (total * HU + gridDim.x - 1) / gridDim.x;
-    if (per < S::kWarps) per = S::kWarps;
-    locate<S::kThreads>(P, scan, per * blockIdx.x, total, &range[0]);
-    locate<S::kThreads>(P, scan, per * (blockIdx.x + 1), total, &range[1]);
-    if (threadIdx.x == 0) P.part_unit[blockIdx.x] = make_int2(-1, 0);
+    if (threadIdx.x <= kW) {
+      const int64_t mine = hi_at - lo;
+      const int w = threadIdx.x;
+      range[w] = list.locate(
+          lo + (mine <= 0x0fffffff ? (int64_t)((uint32_t)mine * w / kW) : mine * w / kW), total);
+    }
   }
   __syncthreads();
-  const Place from = range[0], to = range[1];
+  const Place from = range[warp], to = range[warp + 1];
+  const int units_end = to.unit + (to.tile > 0 ? 1 : 0);  // units met here, the last maybe in part
+  // A unit's length (-1: impossible) and tiles.
+  auto measure = [&](int b, int& len, int& tiles) {
+    const int n = P.cache.seqlens_kv[b];
+    const int64_t most = (int64_t)P.cache.max_pages * P.cache.page_size;
+    len = n >= 0 && n <= most ? n : -1;
+    tiles = len > 0 ? (len - 1) / S::kTile + 1 : 1;
+  };
 
   // The loader: walks this warp's tiles, kStages - 1 ahead of the arithmetic.
-  const uint32_t ring = smem_u32(smem) + warp * S::kStages * S::kStage;
-  Place next = from;  // unit the loader is in; its tiles from next.tile on
-  int next_len = 0, next_end = 0;
-  int next_tile = 0;  // its tile, relative to the start of the CTA's part of the unit
-  auto enter = [&](const Place& p, int& len, int& end) {  // length and last tile in this CTA
-    len = 0;
-    end = 0;
-    if (p.b < P.batch && (p.b < to.b || p.hu < to.hu || (p.hu == to.hu && p.tile < to.tile))) {
-      const int n = P.cache.seqlens_kv[p.b];
-      const int64_t most = (int64_t)P.cache.max_pages * P.cache.page_size;
-      len = n >= 0 && n <= most ? n : -1;
-      end = len > 0 ? (len + kTile - 1) / kTile : 1;
-      if (p.b == to.b && p.hu == to.hu && to.tile < end) end = to.tile;
+  // One warp-wide copy covers 4 rows x 128 bytes, so a lane serves every
+  // fourth row of a tile and its further columns lie at constant distances.
+  const uint32_t ring = smem_u32(smem) + warp * S::kRing;
+  const int lr = lane >> 3, lc = lane & 7;
+  const uint32_t put0 = lr * S::kRowBytes + ((lc ^ lr) << 4);              // rows lr, lr + 8, ..
+  const uint32_t put1 = (lr + 4) * S::kRowBytes + ((lc ^ (lr + 4)) << 4);  // lr + 4, lr + 12, ..
+  int next = from.unit, next_len = 0, next_end = 0;  // the loader's unit
+  int next_tile = from.tile;                         // and tile
+  const int32_t* next_table = nullptr;
+  const uint8_t *next_k = nullptr, *next_v = nullptr;
+  auto open = [&]() {
+    if (next >= units_end) return;
+    const int b = next / HU;
+    const int64_t head = (next - b * HU) / P.chunks * P.cache.head_stride + 16 / S::kElem * lc;
+    next_k = static_cast<const uint8_t*>(P.cache.k) + head * S::kElem;
+    next_v = static_cast<const uint8_t*>(P.cache.v) + head * S::kElem;
+    next_table = P.cache.block_table + b * P.cache.table_stride;
+    measure(b, next_len, next_end);
+    if (next == to.unit) next_end = min(next_end, to.tile);
+  };
+  open();
+  // Lane i holds token i's page number and its row there (-1: no token). They
+  // are fetched a tile ahead of their use, which hides the table's latency.
+  int next_page = 0, next_row = -1;
+  auto look_up = [&]() {  // on to the unit that holds the loader's tile
+    while (next < units_end && next_tile >= next_end) {
+      next_tile = 0;
+      ++next;
+      open();
     }
-  };
-  auto past = [&](Place& p) {  // on to the next unit
-    p.tile = 0;
-    if (++p.hu == HU) {
-      p.hu = 0;
-      ++p.b;
+    const int token = next_tile * S::kTile + lane;
+    next_row = -1;
+    if (next < units_end && lane < S::kTile && token < next_len) {
+      const int in_table = (int)((uint64_t)(uint32_t)token * P.page_mul >> P.page_shift);
+      next_page = next_table[in_table];
+      next_row = token - in_table * P.cache.page_size;
     }
-  };
-  auto beyond = [&](const Place& p) {
-    return p.b > to.b || (p.b == to.b && (p.hu > to.hu || (p.hu == to.hu && p.tile >= to.tile))) ||
-           p.b >= P.batch;
-  };
-  enter(next, next_len, next_end);
-  next_tile = next.tile + warp;
-  auto settle = [&]() {  // to the unit that holds the loader's tile
-    while (!beyond(next) && next_tile >= next_end) {
-      next_tile -= next_end;
-      past(next);
-      enter(next, next_len, next_end);
-    }
-  };
-  settle();
-  int64_t next_off = -1;  // lane < 16: token offset of the loader's tile
-  auto look_up = [&]() {
-    next_off = -1;
-    if (!beyond(next) && lane < kTile)
-      next_off = token_offset(P, next.b, next_tile * kTile + lane, next_len);
   };
   look_up();
   int load_slot = 0;
   auto load = [&]() {
-    if (!beyond(next)) {
-      const uint32_t ok = __ballot_sync(kFullMask, next_off >= 0) & 0xffffu;
+    if (next < units_end) {
+      int64_t off = -1;
+      if (next_row >= 0) {
+        if (next_page >= 0 && next_page < P.cache.num_pages)
+          off = next_page * P.cache.page_stride + (int64_t)next_row * P.cache.token_stride;
+        else
+          report_device_error(P.err, FMHA_ERR_INVALID_ARG, kSiteDecodePage);
+      }
+      const uint32_t ok = __ballot_sync(kFullMask, off >= 0);
       if (lane == 0) tile_mask[warp][load_slot] = ok;
       const uint32_t base = ring + load_slot * S::kStage;
-      const int64_t head = (next.hu / P.chunks) * P.cache.head_stride;
-      const uint8_t* const kb = static_cast<const uint8_t*>(P.cache.k) + head * S::kElem;
-      const uint8_t* const vb = static_cast<const uint8_t*>(P.cache.v) + head * S::kElem;
-      constexpr int kRowsPer = 32 / S::kChunks;  // rows one warp-wide copy covers
 #pragma unroll
-      for (int i = 0; i < kTile / kRowsPer; ++i) {
-        const int r = i * kRowsPer + lane / S::kChunks, ch = lane % S::kChunks;
-        const int64_t off = __shfl_sync(kFullMask, next_off, r);
-        const int64_t src = (off < 0 ? 0 : off) * S::kElem + ch * 16;
-        const uint32_t dst = base + r * S::kRowBytes + ((ch ^ (r & 7)) << 4);
-        cp_async16(dst, kb + src, off < 0 ? 0 : 16);
-        cp_async16(dst + S::kHalf, vb + src, off < 0 ? 0 : 16);
+      for (int i = 0; i < S::kTile / 4; ++i) {
+        const int64_t row = __shfl_sync(kFullMask, off, lr + 4 * i);
+        const int bytes = row < 0 ? 0 : 16;
+        const int64_t at = row < 0 ? 0 : row * S::kElem;
+        const uint32_t dst = base + ((i & 1) ? put1 : put0) + (i >> 1) * 8 * S::kRowBytes;
+#pragma unroll
+        for (int c = 0; c < S::kChunks / 8; ++c) {
+          cp_async16(dst + 128 * c, next_k + at + 128 * c, bytes);
+          cp_async16(dst + 128 * c + S::kHalf, next_v + at + 128 * c, bytes);
+        }
       }
-      next_tile += S::kWarps;
-      settle();
+      ++next_tile;
       look_up();
     }
     cp_async_commit();
@@ -297,37 +329,30 @@ __global__ void __launch_bounds__((DecodeShape<D, F8>::kThreads), 1)
   for (int i = 0; i < S::kStages - 1; ++i) load();
 
   int slot = 0;
-  int turn = 0;  // tiles of this CTA before the current unit's, modulo the warps
-  for (Place p = from; !beyond(p); past(p)) {
-    int len, end;
-    enter(p, len, end);
-    const int first = p.tile;
-    const int tiles = end - first;
-    const int kvh = p.hu / P.chunks, head0 = kvh * P.g + (p.hu % P.chunks) * P.rows;
-    const int rows = min(P.rows, P.g - (p.hu % P.chunks) * P.rows);
-    const bool bad = len < 0;
-    if (bad && threadIdx.x == 0)
-      report_device_error(P.err, FMHA_ERR_INVALID_ARG, kSiteDecodeLength);
-    int mine = warp - turn;  // this warp's first tile here
-    if (mine < 0) mine += S::kWarps;
-    turn = (turn + tiles) % S::kWarps;
+  for (int unit = from.unit; unit < units_end; ++unit) {
+    int len, all;
+    const int b = unit / HU, hu = unit - b * HU;
+    measure(b, len, all);
+    const int first = unit == from.unit ? from.tile : 0;
+    const int end = unit == to.unit ? to.tile : all;
+    const int head0 = hu / P.chunks * P.g + (hu % P.chunks) * P.rows;
+    const int rows = min(P.rows, P.g - (hu % P.chunks) * P.rows);
 
     // Query fragments: row gr (and gr + 8). Element order along head_dim is
     // the one K's fragments come in: natural for 16-bit rows, and for e4m3
     // rows 4c..4c+3 of each 16 (two to each half of the MMA's 16).
-    uint32_t qa[kSteps][WIDE ? 4 : 2];
-    float qs[WIDE ? 2 : 1];  // per-row factor of the scores
+    uint32_t qa[kSteps][2 * kH];
+    float qs[kH];  // per-row factor of the scores
 #pragma unroll
-    for (int half = 0; half < (WIDE ? 2 : 1); ++half) {
+    for (int half = 0; half < kH; ++half) {
       const int row = gr + 8 * half;
       const bool have = row < rows;
-      const uint16_t* const src =
-          P.q + p.b * P.q_stride + (int64_t)(head0 + (have ? row : 0)) * D;
+      const uint16_t* const src = P.q + b * P.q_stride + (int64_t)(head0 + (have ? row : 0)) * D;
       qs[half] = P.scale_log2;
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         uint32_t w0 = 0, w1 = 0;
-        if (have && mine < tiles) {
+        if (have) {
           if constexpr (F8) {
             const uint2 w = *reinterpret_cast<const uint2*>(src + 16 * s + 4 * gc);
             w0 = w.x;
@@ -338,7 +363,7 @@ __global__ void __launch_bounds__((DecodeShape<D, F8>::kThreads), 1)
           }
         }
         qa[s][half] = w0;
-        qa[s][(WIDE ? 2 : 1) + half] = w1;
+        qa[s][kH + half] = w1;
       }
       if constexpr (F8 && BF16) {
         // bf16 -> fp16: the row times 2^e, e such that its largest element
@@ -351,7 +376,7 @@ __global__ void __launch_bounds__((DecodeShape<D, F8>::kThreads), 1)
         for (int s = 0; s < kSteps; ++s)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float2 f = unpack2<true>(qa[s][j * (WIDE ? 2 : 1) + half]);
+            const float2 f = unpack2<true>(qa[s][j * kH + half]);
             top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
             odd |= !(fabsf(f.x) <= FLT_MAX) || !(fabsf(f.y) <= FLT_MAX);
           }
@@ -368,7 +393,7 @@ __global__ void __launch_bounds__((DecodeShape<D, F8>::kThreads), 1)
         for (int s = 0; s < kSteps; ++s)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            uint32_t& w = qa[s][j * (WIDE ? 2 : 1) + half];
+            uint32_t& w = qa[s][j * kH + half];
             const float2 f = unpack2<true>(w);
             w = pack2<false>(f.x * up, f.y * up);
           }
@@ -380,14 +405,14 @@ __global__ void __launch_bounds__((DecodeShape<D, F8>::kThreads), 1)
     for (int i = 0; i < D / 8; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-    float m[WIDE ? 2 : 1], l[WIDE ? 2 : 1];
+    float m[kH], l[kH];
 #pragma unroll
-    for (int h = 0; h < (WIDE ? 2 : 1); ++h) {
+    for (int h = 0; h < kH; ++h) {
       m[h] = -INFINITY;
       l[h] = 0.0f;
     }
 
-    for (int t = mine; t < tiles; t += S::kWarps) {
+    for (int t = first; t < end; ++t) {
       cp_async_wait<S::kStages - 2>();
       __syncwarp();
       load();  // into the slot of the tile before this one
@@ -395,27 +420,30 @@ __global__ void __launch_bounds__((DecodeShape<D, F8>::kThreads), 1)
       const uint32_t ok = tile_mask[warp][slot];
       slot = slot + 1 == S::kStages ? 0 : slot + 1;
 
-      // Scores of 16 tokens: two 8-token column tiles.
-      float sc[2][4] = {};
+      // Scores of the tile's tokens, 8 to a column tile.
+      float sc[2 * S::kSub][4] = {};
       if constexpr (F8) {
         // One ldmatrix.x4: 16 tokens x 32 bytes; each lane gets 4 adjacent
         // codes of its token per 16 bytes.
 #pragma unroll
         for (int s = 0; s < kSteps; s += 2) {
           const int r = (lane & 7) + ((lane >> 4) << 3), ch = s + ((lane >> 3) & 1);
-          uint32_t w[4];
-          ldsm4(w, kt + r * S::kRowBytes + ((ch ^ (r & 7)) << 4));
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+          for (int u = 0; u < S::kSub; ++u) {
+            uint32_t w[4];
+            ldsm4(w, kt + (16 * u + r) * S::kRowBytes + ((ch ^ (r & 7)) << 4));
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const uint32_t x = w[2 * n + j];
-              const uint32_t b0 = e4m3x2_to_half2(x & 0xffffu), b1 = e4m3x2_to_half2(x >> 16);
-              if constexpr (WIDE)
-                mma16<kB>(sc[n], qa[s + j][0], qa[s + j][1], qa[s + j][2], qa[s + j][3], b0, b1);
-              else
-                mma16<kB>(sc[n], qa[s + j][0], 0u, qa[s + j][1], 0u, b0, b1);
-            }
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const uint32_t x = w[2 * n + j];
+                const uint32_t b0 = e4m3x2_to_half2(x & 0xffffu), b1 = e4m3x2_to_half2(x >> 16);
+                if constexpr (WIDE)
+                  mma16<kB>(sc[2 * u + n], qa[s + j][0], qa[s + j][1], qa[s + j][2], qa[s + j][3], b0, b1);
+                else
+                  mma16<kB>(sc[2 * u + n], qa[s + j][0], 0u, qa[s + j][1], 0u, b0, b1);
+              }
+          }
         }
       } else {
 #pragma unroll
@@ -434,39 +462,47 @@ __global__ void __launch_bounds__((DecodeShape<D, F8>::kThreads), 1)
       }
 
       // Running maximum, and P as two 16-bit parts in A-fragment order.
-      uint32_t hi[2][2], lo[2][2];  // [row half][column tile]
-      float down[WIDE ? 2 : 1];
+      uint32_t hi[kH][2 * S::kSub], lo[kH][2 * S::kSub];  // [row half][column tile]
+      float down[kH];
       bool rose = false;
 #pragma unroll
-      for (int h = 0; h < (WIDE ? 2 : 1); ++h) {
-        float s4[4];
+      for (int h = 0; h < kH; ++h) {
+        constexpr int kN = 4 * S::kSub;
+        float x[kN];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int i = 0; i < kN; ++i) x[i] = sc[i >> 1][2 * h + (i & 1)] * qs[h];
+        if (ok != (S::kTile == 32 ? 0xffffffffu : 0xffffu)) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-            s4[2 * n + j] = (ok >> (8 * n + 2 * gc + j)) & 1u ? sc[n][2 * h + j] * qs[h] : -INFINITY;
-        float top = fmaxf(fmaxf(s4[0], s4[1]), fmaxf(s4[2], s4[3]));
+          for (int i = 0; i < kN; ++i)
+            if (!((ok >> (8 * (i >> 1) + 2 * gc + (i & 1))) & 1u)) x[i] = -INFINITY;
+        }
+        float top = x[0];
+#pragma unroll
+        for (int i = 1; i < kN; ++i) top = fmaxf(top, x[i]);
         top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 1));
         top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 2));
         const float now = fmaxf(m[h], top);
         const float ref = now == -INFINITY ? 0.0f : now;  // nothing seen yet: weights 2^-inf = 0
-        down[h] = exp2f(m[h] - ref);
+        down[h] = ex2(m[h] - ref);
         rose |= now != m[h];
         m[h] = now;
-        float pr[4];
+        float sum = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) pr[j] = exp2f(s4[j] - (ref - kShift));
-        l[h] = l[h] * down[h] + ((pr[0] + pr[1]) + (pr[2] + pr[3]));
-        split2<kB>(pr[0], pr[1], hi[h][0], lo[h][0]);
-        split2<kB>(pr[2], pr[3], hi[h][1], lo[h][1]);
+        for (int i = 0; i < kN; ++i) {
+          x[i] = ex2(x[i] - (ref - kShift));
+          sum += x[i];
+        }
+        l[h] = l[h] * down[h] + sum;
+#pragma unroll
+        for (int i = 0; i < kN / 2; ++i) split2<kB>(x[2 * i], x[2 * i + 1], hi[h][i], lo[h][i]);
       }
       if (__any_sync(kFullMask, rose)) {
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
           acc[i][0] *= down[0];
           acc[i][1] *= down[0];
-          acc[i][2] *= down[WIDE ? 1 : 0];
-          acc[i][3] *= down[WIDE ? 1 : 0];
+          acc[i][2] *= down[kH - 1];
+          acc[i][3] *= down[kH - 1];
         }
       }
 
@@ -474,112 +510,183 @@ __global__ void __launch_bounds__((DecodeShape<D, F8>::kThreads), 1)
 #pragma unroll
       for (int i = 0; i < S::kChunks; i += 2) {
         const int r = (lane & 7) + (((lane >> 3) & 1) << 3), ch = i + (lane >> 4);
-        uint32_t w[4];
-        ldsm4_trans(w, vt + r * S::kRowBytes + ((ch ^ (r & 7)) << 4));
-        auto pv = [&](float (&a)[4], uint32_t b0, uint32_t b1) {
-          if constexpr (WIDE) {
-            mma16<kB>(a, hi[0][0], hi[1][0], hi[0][1], hi[1][1], b0, b1);
-            mma16<kB>(a, lo[0][0], lo[1][0], lo[0][1], lo[1][1], b0, b1);
-          } else {
-            mma16<kB>(a, hi[0][0], lo[0][0], hi[0][1], lo[0][1], b0, b1);
-          }
-        };
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          if constexpr (F8) {
-            // Each 32-bit word: two tokens x two adjacent columns; tile 2k
-            // takes the even columns of a 16-byte piece, tile 2k+1 the odd.
-            const uint32_t x = w[2 * j], y = w[2 * j + 1];
-            pv(acc[2 * (i + j)], e4m3x2_to_half2(__byte_perm(x, 0, 0x4420)),
-               e4m3x2_to_half2(__byte_perm(y, 0, 0x4420)));
-            pv(acc[2 * (i + j) + 1], e4m3x2_to_half2(__byte_perm(x, 0, 0x4431)),
-               e4m3x2_to_half2(__byte_perm(y, 0, 0x4431)));
-          } else {
-            pv(acc[i + j], w[2 * j], w[2 * j + 1]);
+        for (int u = 0; u < S::kSub; ++u) {
+          uint32_t w[4];
+          ldsm4_trans(w, vt + (16 * u + r) * S::kRowBytes + ((ch ^ (r & 7)) << 4));
+          auto pv = [&](float (&a)[4], uint32_t b0, uint32_t b1) {
+            if constexpr (WIDE) {
+              mma16<kB>(a, hi[0][2 * u], hi[1][2 * u], hi[0][2 * u + 1], hi[1][2 * u + 1], b0, b1);
+              mma16<kB>(a, lo[0][2 * u], lo[1][2 * u], lo[0][2 * u + 1], lo[1][2 * u + 1], b0, b1);
+            } else {
+              mma16<kB>(a, hi[0][2 * u], lo[0][2 * u], hi[0][2 * u + 1], lo[0][2 * u + 1], b0, b1);
+            }
+          };
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            if constexpr (F8) {
+              // Each 32-bit word: two tokens x two adjacent columns; tile 2k
+              // takes the even columns of a 16-byte piece, tile 2k+1 the odd.
+              const uint32_t x = w[2 * j], y = w[2 * j + 1];
+              pv(acc[2 * (i + j)], e4m3x2_to_half2(__byte_perm(x, 0, 0x4420)),
+                 e4m3x2_to_half2(__byte_perm(y, 0, 0x4420)));
+              pv(acc[2 * (i + j) + 1], e4m3x2_to_half2(__byte_perm(x, 0, 0x4431)),
+                 e4m3x2_to_half2(__byte_perm(y, 0, 0x4431)));
+            } else {
+              pv(acc[i + j], w[2 * j], w[2 * j + 1]);
+            }
           }
         }
       }
     }
 
-    // Join across the warps. Rows 8..15 of a narrow group hold the low parts.
+    // The unit's result so far: rows 8..15 of a narrow group hold low parts.
 #pragma unroll
-    for (int h = 0; h < (WIDE ? 2 : 1); ++h) {
+    for (int h = 0; h < kH; ++h) {
       l[h] += __shfl_xor_sync(kFullMask, l[h], 1);
       l[h] += __shfl_xor_sync(kFullMask, l[h], 2);
-      if (gc == 0) join_ml[warp][gr + 8 * h] = make_float2(m[h], l[h]);
     }
-    const bool starts = first == 0;
-    const bool ends = P.whole || bad || end == (len > 0 ? (len + kTile - 1) / kTile : 1);
-    const int part = starts ? 1 : 0;  // a unit that began earlier lies in part 0
-    if (!(starts && ends) && threadIdx.x == 0 && starts) {
-      // The CTA that holds the unit's last tile, from the even deal.
-      const int n = (len + kTile - 1) / kTile;
-      const int64_t here = per * (blockIdx.x + 1);  // tile number of this CTA's end
-      const int64_t last = here + (n - end) - 1;
-      P.part_unit[blockIdx.x] = make_int2(p.b * HU + p.hu, (int)(last / per));
+    const bool done = first == 0 && end == all;
+    if (len < 0) {
+      if (lane == 0) report_device_error(P.err, FMHA_ERR_INVALID_ARG, kSiteDecodeLength);
+      continue;
     }
-    float* const jo = reinterpret_cast<float*>(smem + S::kRing);
+    const int keep = 2 * warp + (first == 0 ? 1 : 0);
+    float* const held = reinterpret_cast<float*>(
+        smem + (first == 0 ? warp * S::kRing : kW * S::kRing + warp * S::kHold));
+    if (!done) {
+      // Its tiles are read and, where the unit goes on behind this warp's
+      // range, no more are loaded: the ring may take the result.
+      __syncwarp();
+      if (lane == 0) {
+        slot_unit[keep] = unit;
+        slot_ends[keep] = end == all;
+      }
+    }
 #pragma unroll
-    for (int h = 0; h < (WIDE ? 2 : 1); ++h) {
-      if (h == 1) __syncthreads();  // the rows before are out of the buffer
-      float* const row = jo + (warp * 8 + gr) * S::kPad;
+    for (int h = 0; h < kH; ++h) {
+      const int row = gr + 8 * h;
+      const float inv = len == 0 ? 0.0f : P.cache.v_scale / l[h];  // 0/0 where every score is -inf
+      if (!done && gc == 0) slot_ml[keep][row] = make_float2(m[h], l[h]);
+      if (done && row < rows && gc == 0 && P.lse)
+        P.lse[(int64_t)b * P.hkv * P.g + head0 + row] =
+            (m[h] + (log2f(l[h]) - kShift)) * 0.69314718055994531f;
+      uint16_t* const out = P.o + b * P.o_stride + (int64_t)(head0 + row) * D;
+      auto value = [&](int i, int j) {
+        return WIDE ? acc[i][2 * h + j] : acc[i][j] + acc[i][j + 2];
+      };
+      auto pack = [&](float x, float y) {
+        return P.o_bf16 ? pack2<true>(x * inv, y * inv) : pack2<false>(x * inv, y * inv);
+      };
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        float x0, x1;
-        if constexpr (WIDE) {
-          x0 = acc[i][2 * h];
-          x1 = acc[i][2 * h + 1];
-        } else {
-          x0 = acc[i][0] + acc[i][2];
-          x1 = acc[i][1] + acc[i][3];
-        }
+      for (int i = 0; i < D / 8; i += F8 ? 2 : 1) {
         if constexpr (F8) {
           // tile 2k + e, column n -> head_dim 16k + 2n + e
-          row[16 * (i / 2) + 4 * gc + (i & 1)] = x0;
-          row[16 * (i / 2) + 4 * gc + 2 + (i & 1)] = x1;
+          const int d = 8 * i + 4 * gc;
+          const float x0 = value(i, 0), x1 = value(i + 1, 0), x2 = value(i, 1), x3 = value(i + 1, 1);
+          if (!done)
+            *reinterpret_cast<float4*>(held + row * S::kPad + d) = make_float4(x0, x1, x2, x3);
+          else if (row < rows)
+            *reinterpret_cast<uint2*>(out + d) = make_uint2(pack(x0, x1), pack(x2, x3));
         } else {
-          *reinterpret_cast<float2*>(row + 8 * i + 2 * gc) = make_float2(x0, x1);
-        }
-      }
-      __syncthreads();
-      const int here = min(8, rows - 8 * h);
-      for (int e = threadIdx.x * 2; e < here * D; e += 2 * S::kThreads) {
-        const int r = e / D, d = e % D;
-        float top = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < S::kWarps; ++w) top = fmaxf(top, join_ml[w][8 * h + r].x);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        float sum = 0.0f, x0 = 0.0f, x1 = 0.0f;
-#pragma unroll
-        for (int w = 0; w < S::kWarps; ++w) {
-          const float2 ml = join_ml[w][8 * h + r];
-          const float f = exp2f(ml.x - ref);
-          const float2 v = *reinterpret_cast<const float2*>(jo + (w * 8 + r) * S::kPad + d);
-          sum += ml.y * f;
-          x0 += v.x * f;
-          x1 += v.y * f;
-        }
-        if (bad) continue;
-        if (starts && ends) {
-          const float inv = P.cache.v_scale / sum;  // 0/0 where every score is -inf
-          x0 = len == 0 ? 0.0f : x0 * inv;
-          x1 = len == 0 ? 0.0f : x1 * inv;
-          uint32_t* const out = reinterpret_cast<uint32_t*>(
-              P.o + p.b * P.o_stride + (int64_t)(head0 + 8 * h + r) * D + d);
-          *out = P.o_bf16 ? pack2<true>(x0, x1) : pack2<false>(x0, x1);
-          if (P.lse && d == 0)
-            P.lse[(int64_t)p.b * P.hkv * P.g + head0 + 8 * h + r] =
-                (top + (log2f(sum) - kShift)) * 0.69314718055994531f;
-        } else {
-          const int64_t at = ((int64_t)blockIdx.x * 2 + part) * P.rows + 8 * h + r;
-          *reinterpret_cast<float2*>(P.part_o + at * D + d) = make_float2(x0, x1);
-          if (d == 0) P.part_ml[at] = make_float2(top, sum);
+          const int d = 8 * i + 2 * gc;
+          const float x0 = value(i, 0), x1 = value(i, 1);
+          if (!done)
+            *reinterpret_cast<float2*>(held + row * S::kPad + d) = make_float2(x0, x1);
+          else if (row < rows)
+            *reinterpret_cast<uint32_t*>(out + d) = pack(x0, x1);
         }
       }
     }
-    __syncthreads();
   }
   cp_async_wait<0>();
+  __syncthreads();
+
+  // Joins the CTA's held results, unit by unit; the rows of all of them are
+  // dealt to the warps in turn. Lane e looks after slot e.
+  const Place cta_end = range[kW];
+  const int my_unit = lane < 2 * kW ? slot_unit[lane] : -1;
+  const unsigned alike = __match_any_sync(kFullMask, my_unit);
+  unsigned firsts = __ballot_sync(kFullMask, my_unit >= 0 && (alike & ((1u << lane) - 1)) == 0);
+  int turn = warp;
+  while (firsts) {
+    const int s0 = __ffs(firsts) - 1;
+    firsts &= firsts - 1;
+    if (turn >= P.rows) {  // none of its rows is this warp's
+      turn -= P.rows;
+      continue;
+    }
+    const int unit = __shfl_sync(kFullMask, my_unit, s0);
+    const unsigned slots = __shfl_sync(kFullMask, alike, s0);
+    const bool starts = (s0 & 1) != 0;  // held as a warp's last unit: it began there
+    const bool ends = slot_ends[31 - __clz(slots)] != 0;
+    const int b = unit / HU, hu = unit - b * HU;
+    const int head0 = hu / P.chunks * P.g + (hu % P.chunks) * P.rows;
+    const int rows = min(P.rows, P.g - (hu % P.chunks) * P.rows);
+    if (starts && !ends && turn == 0 && lane == 0) {
+      // It goes on in the next CTA: the CTA of its last tile, from the even deal.
+      int len, all;
+      measure(b, len, all);
+      P.part_unit[blockIdx.x] = make_int2(unit, (int)((hi_at - cta_end.tile + all - 1) / per));
+    }
+    int r = turn;
+    for (; r < rows; r += kW) {
+      float2 ml = make_float2(-INFINITY, 0.0f);
+      if ((slots >> lane) & 1u) ml = slot_ml[lane][r];
+      float top = ml.x;
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o, 16));
+      top = __shfl_sync(kFullMask, top, 0);
+      const float ref = top == -INFINITY ? 0.0f : top;
+      const float f = ex2(ml.x - ref);
+      float sum = ml.y * f;
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o, 16);
+      sum = __shfl_sync(kFullMask, sum, 0);
+      float4 x[D / 128];
+#pragma unroll
+      for (int i = 0; i < D / 128; ++i) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (unsigned left = slots; left; left &= left - 1) {
+        const int e = __ffs(left) - 1;
+        const float fe = __shfl_sync(kFullMask, f, e);
+        const float* const held =
+            reinterpret_cast<const float*>(smem + ((e & 1) ? (e >> 1) * S::kRing
+                                                           : kW * S::kRing + (e >> 1) * S::kHold)) +
+            r * S::kPad;
+#pragma unroll
+        for (int i = 0; i < D / 128; ++i) {
+          const float4 y = *reinterpret_cast<const float4*>(held + 128 * i + 4 * lane);
+          x[i].x += y.x * fe;
+          x[i].y += y.y * fe;
+          x[i].z += y.z * fe;
+          x[i].w += y.w * fe;
+        }
+      }
+      if (starts && ends) {
+        const float inv = P.cache.v_scale / sum;
+        uint16_t* const out = P.o + b * P.o_stride + (int64_t)(head0 + r) * D + 4 * lane;
+#pragma unroll
+        for (int i = 0; i < D / 128; ++i) {
+          const float4 y = make_float4(x[i].x * inv, x[i].y * inv, x[i].z * inv, x[i].w * inv);
+          *reinterpret_cast<uint2*>(out + 128 * i) =
+              P.o_bf16 ? make_uint2(pack2<true>(y.x, y.y), pack2<true>(y.z, y.w))
+                       : make_uint2(pack2<false>(y.x, y.y), pack2<false>(y.z, y.w));
+        }
+        if (P.lse && lane == 0)
+          P.lse[(int64_t)b * P.hkv * P.g + head0 + r] =
+              (top + (log2f(sum) - kShift)) * 0.69314718055994531f;
+      } else {
+        const int64_t at = ((int64_t)blockIdx.x * 2 + (starts ? 1 : 0)) * P.rows + r;
+#pragma unroll
+        for (int i = 0; i < D / 128; ++i)
+          *reinterpret_cast<float4*>(P.part_o + at * D + 128 * i + 4 * lane) = x[i];
+        if (lane == 0) P.part_ml[at] = make_float2(top, sum);
+      }
+    }
+    while (r < P.rows) r += kW;
+    turn = r - P.rows;
+  }
 }
 
 // Joins the parts of the unit that starts in CTA blockIdx.x and ends in a
@@ -612,7 +719,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     const float2 ml = P.part_ml[at];
     const float now = fmaxf(m, ml.x);
     const float ref = now == -INFINITY ? 0.0f : now;
-    const float f0 = exp2f(m - ref), f1 = exp2f(ml.x - ref);
+    const float f0 = ex2(m - ref), f1 = ex2(ml.x - ref);
     m = now;
     l = l * f0 + ml.y * f1;
 #pragma unroll
@@ -638,7 +745,7 @@ __global__ void __launch_bounds__(kJoinThreads)
   float sum = 0.0f, x0 = 0.0f, x1 = 0.0f;
 #pragma unroll
   for (int w = 0; w < kJoinThreads / 32; ++w) {
-    const float f = exp2f(warp_ml[w].x - ref);
+    const float f = ex2(warp_ml[w].x - ref);
     sum += warp_ml[w].y * f;
     x0 += warp_o[w][d] * f;
     x1 += warp_o[w][d + 1] * f;
@@ -652,24 +759,22 @@ __global__ void __launch_bounds__(kJoinThreads)
 
 using DecodeFn = void (*)(const DecodeParams);
 
-template <int D, bool BF16, bool F8>
-DecodeFn decode_fn_wide(bool wide) {
-  return wide ? paged_decode_kernel<D, BF16, F8, true> : paged_decode_kernel<D, BF16, F8, false>;
+struct DecodeLaunch {
+  DecodeFn fn;
+  int smem, threads;
+};
+
+template <int D, bool F8, bool WIDE>
+DecodeLaunch decode_launch(bool bf16) {
+  using S = DecodeShape<D, F8, WIDE>;
+  return {bf16 ? paged_decode_kernel<D, true, F8, WIDE> : paged_decode_kernel<D, false, F8, WIDE>,
+          S::kSmem, S::kThreads};
 }
 
 template <int D>
-DecodeFn decode_fn(bool bf16, bool f8, bool wide) {
-  if (bf16) return f8 ? decode_fn_wide<D, true, true>(wide) : decode_fn_wide<D, true, false>(wide);
-  return f8 ? decode_fn_wide<D, false, true>(wide) : decode_fn_wide<D, false, false>(wide);
-}
-
-template <int D>
-int decode_smem(bool f8) {
-  return f8 ? DecodeShape<D, true>::kSmem : DecodeShape<D, false>::kSmem;
-}
-template <int D>
-int decode_threads(bool f8) {
-  return f8 ? DecodeShape<D, true>::kThreads : DecodeShape<D, false>::kThreads;
+DecodeLaunch decode_launch(bool bf16, bool f8, bool wide) {
+  if (f8) return wide ? decode_launch<D, true, true>(bf16) : decode_launch<D, true, false>(bf16);
+  return wide ? decode_launch<D, false, true>(bf16) : decode_launch<D, false, false>(bf16);
 }
 
 // Query heads of a unit, and the units of a kv head.
@@ -678,8 +783,11 @@ void unit_rows(int g, int* rows, int* chunks) {
   *rows = (g + *chunks - 1) / *chunks;
 }
 
+bool takes_whole_units(int64_t max_tokens) { return max_tokens <= kWholeTokens; }
+
 // The workspace: partial outputs, then (m, l), then the units to join.
-int64_t workspace_bytes_for(int rows, int d) {
+int64_t workspace_bytes_for(int rows, int d, int64_t max_tokens) {
+  if (takes_whole_units(max_tokens)) return 0;
   return (int64_t)kMaxCtas * 2 * rows * (d * 4 + 8) + (int64_t)kMaxCtas * 8;
 }
 
@@ -688,76 +796,80 @@ int64_t workspace_bytes_for(int rows, int d) {
 
 using namespace fmha;
 
-extern "C" int64_t fmha_paged_decode_workspace(int num_heads_q, int num_heads_kv, int head_dim) {
-  if (check_heads(num_heads_q, num_heads_kv, head_dim) != FMHA_OK) return -1;
+extern "C" int64_t fmha_paged_decode_workspace(int num_heads_q, int num_heads_kv, int head_dim,
+                                               int64_t max_tokens) {
+  if (check_heads(num_heads_q, num_heads_kv, head_dim) != FMHA_OK || max_tokens < 0) return -1;
   int rows, chunks;
   unit_rows(num_heads_q / num_heads_kv, &rows, &chunks);
-  return workspace_bytes_for(rows, head_dim);
+  return workspace_bytes_for(rows, head_dim, max_tokens);
 }
 
-extern "C" fmha_status_t fmha_paged_decode(const void* Q, const fmha_paged_cache_t* cache, void* O,
-                                           float* LSE, int batch, int num_heads_q,
-                                           int num_heads_kv, int head_dim, int64_t q_stride,
-                                           int64_t o_stride, float softmax_scale, int dtype,
-                                           int o_dtype, void* workspace, int64_t workspace_bytes,
+extern "C" fmha_status_t fmha_paged_decode(const fmha_paged_decode_args_t* args,
                                            fmha_stream_t stream) {
+  if (!args) return FMHA_ERR_INVALID_ARG;
+  const fmha_paged_decode_args_t& A = *args;
+  const int batch = A.batch, d = A.head_dim;
   if (batch < 0) return FMHA_ERR_INVALID_ARG;
-  fmha_status_t st = check_heads(num_heads_q, num_heads_kv, head_dim);
+  fmha_status_t st = check_heads(A.num_heads_q, A.num_heads_kv, d);
   if (st != FMHA_OK) return st;
-  if (dtype != FMHA_DTYPE_BF16 && dtype != FMHA_DTYPE_FP16) return FMHA_ERR_UNSUPPORTED;
-  if (o_dtype != FMHA_DTYPE_BF16 && o_dtype != FMHA_DTYPE_FP16) return FMHA_ERR_UNSUPPORTED;
-  if (!(softmax_scale >= 0.0f) || std::isinf(softmax_scale)) return FMHA_ERR_INVALID_ARG;
+  if (A.dtype != FMHA_DTYPE_BF16 && A.dtype != FMHA_DTYPE_FP16) return FMHA_ERR_UNSUPPORTED;
+  if (A.o_dtype != FMHA_DTYPE_BF16 && A.o_dtype != FMHA_DTYPE_FP16) return FMHA_ERR_UNSUPPORTED;
+  if (!(A.softmax_scale >= 0.0f) || std::isinf(A.softmax_scale)) return FMHA_ERR_INVALID_ARG;
   if (batch == 0) return FMHA_OK;
-  if ((st = check_rows(Q, q_stride, num_heads_q, head_dim)) != FMHA_OK ||
-      (st = check_rows(O, o_stride, num_heads_q, head_dim)) != FMHA_OK)
+  if ((st = check_rows(A.q, A.q_stride, A.num_heads_q, d)) != FMHA_OK ||
+      (st = check_rows(A.o, A.o_stride, A.num_heads_q, d)) != FMHA_OK)
     return st;
   DecodeParams P;
   std::memset(&P, 0, sizeof(P));
-  if ((st = check_cache(cache, num_heads_kv, head_dim, dtype, &P.cache)) != FMHA_OK) return st;
-  if (reinterpret_cast<uintptr_t>(LSE) & 3u) return FMHA_ERR_MISALIGNED;
-  P.g = num_heads_q / num_heads_kv;
+  if ((st = check_cache(A.cache, A.num_heads_kv, d, A.dtype, &P.cache)) != FMHA_OK) return st;
+  if (reinterpret_cast<uintptr_t>(A.lse) & 3u) return FMHA_ERR_MISALIGNED;
+  P.g = A.num_heads_q / A.num_heads_kv;
   unit_rows(P.g, &P.rows, &P.chunks);
-  if (!workspace || workspace_bytes < workspace_bytes_for(P.rows, head_dim))
-    return FMHA_ERR_INVALID_ARG;
-  if (!aligned16(workspace)) return FMHA_ERR_MISALIGNED;
-  if ((int64_t)batch * num_heads_kv * P.chunks > (int64_t)1 << 30) return FMHA_ERR_UNSUPPORTED;
+  const int64_t longest = (int64_t)P.cache.max_pages * P.cache.page_size;  // tokens
+  P.whole = takes_whole_units(longest);
+  if (!P.whole) {
+    if (!A.workspace || A.workspace_bytes < workspace_bytes_for(P.rows, d, longest))
+      return FMHA_ERR_INVALID_ARG;
+    if (!aligned16(A.workspace)) return FMHA_ERR_MISALIGNED;
+  }
+  const int64_t units = (int64_t)batch * A.num_heads_kv * P.chunks;
+  if (units > (int64_t)1 << 30) return FMHA_ERR_UNSUPPORTED;
   ServingDevice dev;
   if ((st = serving_device(&dev)) != FMHA_OK) return st;
-  P.q = static_cast<const uint16_t*>(Q);
-  P.o = static_cast<uint16_t*>(O);
-  P.lse = LSE;
+  P.q = static_cast<const uint16_t*>(A.q);
+  P.o = static_cast<uint16_t*>(A.o);
+  P.lse = A.lse;
   P.batch = batch;
-  P.hkv = num_heads_kv;
-  P.q_stride = q_stride;
-  P.o_stride = o_stride;
+  P.hkv = A.num_heads_kv;
+  P.q_stride = A.q_stride;
+  P.o_stride = A.o_stride;
   const double scale =
-      softmax_scale > 0.0f ? (double)softmax_scale : 1.0 / std::sqrt((double)head_dim);
+      A.softmax_scale > 0.0f ? (double)A.softmax_scale : 1.0 / std::sqrt((double)d);
   P.scale_log2 = (float)(1.4426950408889634 * scale * P.cache.k_scale);
-  P.o_bf16 = o_dtype == FMHA_DTYPE_BF16;
+  P.o_bf16 = A.o_dtype == FMHA_DTYPE_BF16;
   P.err = dev.err;
-  const int64_t units = (int64_t)batch * num_heads_kv * P.chunks;
-  const int64_t longest = (int64_t)P.cache.max_pages * P.cache.page_size;  // tokens
-  P.whole = longest <= kWholeTiles * kTile;
+  int log2_up = 0;
+  while (((int64_t)1 << log2_up) < P.cache.page_size) ++log2_up;
+  P.page_shift = 31 + log2_up;
+  P.page_mul = (uint32_t)((((uint64_t)1 << P.page_shift) + P.cache.page_size - 1) / P.cache.page_size);
   int ctas = dev.sms < kMaxCtas ? dev.sms : kMaxCtas;
   if (P.whole && units < ctas) ctas = (int)units;
-  char* w = static_cast<char*>(workspace);
+  char* w = static_cast<char*>(A.workspace);
   P.part_o = reinterpret_cast<float*>(w);
-  w += (int64_t)kMaxCtas * 2 * P.rows * head_dim * 4;
+  w += (int64_t)kMaxCtas * 2 * P.rows * d * 4;
   P.part_ml = reinterpret_cast<float2*>(w);
   w += (int64_t)kMaxCtas * 2 * P.rows * 8;
   P.part_unit = reinterpret_cast<int2*>(w);
 
   const bool f8 = P.cache.dtype == FMHA_DTYPE_E4M3, wide = P.rows > 8;
-  const bool bf16 = dtype == FMHA_DTYPE_BF16;
+  const bool bf16 = A.dtype == FMHA_DTYPE_BF16;
   P.shift = bf16 && !f8 ? weight_shift<true, false>() : weight_shift<false, false>();
-  const DecodeFn fn = head_dim == 128 ? decode_fn<128>(bf16, f8, wide)
-                                      : decode_fn<256>(bf16, f8, wide);
-  const int smem = head_dim == 128 ? decode_smem<128>(f8) : decode_smem<256>(f8);
-  const int threads = head_dim == 128 ? decode_threads<128>(f8) : decode_threads<256>(f8);
-  if ((st = ensure_smem(reinterpret_cast<const void*>(fn), smem)) != FMHA_OK) return st;
+  const DecodeLaunch how = d == 128 ? decode_launch<128>(bf16, f8, wide)
+                                    : decode_launch<256>(bf16, f8, wide);
+  if ((st = ensure_smem(reinterpret_cast<const void*>(how.fn), how.smem)) != FMHA_OK) return st;
   const cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
-  st = launch_serving(fn, dim3(ctas), threads, smem, cs, P);
+  st = launch_serving(how.fn, dim3(ctas), how.threads, how.smem, cs, P);
   if (st != FMHA_OK || P.whole) return st;
-  return launch_serving(head_dim == 128 ? paged_join_kernel<128> : paged_join_kernel<256>,
+  return launch_serving(d == 128 ? paged_join_kernel<128> : paged_join_kernel<256>,
                         dim3(ctas, P.rows), kJoinThreads, 0, cs, P);
 }

@@ -652,77 +652,74 @@ bool encode(CUtensorMap* map, bool bf16, const void* p, int d, int heads, int ro
 
 using namespace fmha;
 
-extern "C" fmha_status_t fmha_prompt(const void* Q, const void* K, const void* V, void* O,
-                                     float* LSE, const int32_t* cu_seqlens_q,
-                                     const int32_t* cu_seqlens_kv, int total_q, int total_kv,
-                                     int batch, int num_heads_q, int num_heads_kv, int head_dim,
-                                     int64_t q_stride, int64_t k_stride, int64_t v_stride,
-                                     int64_t o_stride, float softmax_scale, int causal, int dtype,
-                                     int o_dtype, fmha_stream_t stream) {
-  if (total_q < 0 || total_kv < 0 || batch < 0) return FMHA_ERR_INVALID_ARG;
-  fmha_status_t st = check_heads(num_heads_q, num_heads_kv, head_dim);
+extern "C" fmha_status_t fmha_prompt(const fmha_prompt_args_t* args, fmha_stream_t stream) {
+  if (!args) return FMHA_ERR_INVALID_ARG;
+  const fmha_prompt_args_t& A = *args;
+  if (A.total_q < 0 || A.total_kv < 0 || A.batch < 0) return FMHA_ERR_INVALID_ARG;
+  const int hq = A.num_heads_q, hkv = A.num_heads_kv, d = A.head_dim;
+  fmha_status_t st = check_heads(hq, hkv, d);
   if (st != FMHA_OK) return st;
-  if (dtype != FMHA_DTYPE_BF16 && dtype != FMHA_DTYPE_FP16) return FMHA_ERR_UNSUPPORTED;
-  if (o_dtype != FMHA_DTYPE_BF16 && o_dtype != FMHA_DTYPE_FP16) return FMHA_ERR_UNSUPPORTED;
-  if (!(softmax_scale >= 0.0f) || std::isinf(softmax_scale)) return FMHA_ERR_INVALID_ARG;
-  if (total_q == 0 || batch == 0) return FMHA_OK;
-  if ((st = check_rows(Q, q_stride, num_heads_q, head_dim)) != FMHA_OK ||
-      (st = check_rows(O, o_stride, num_heads_q, head_dim)) != FMHA_OK)
+  if (A.dtype != FMHA_DTYPE_BF16 && A.dtype != FMHA_DTYPE_FP16) return FMHA_ERR_UNSUPPORTED;
+  if (A.o_dtype != FMHA_DTYPE_BF16 && A.o_dtype != FMHA_DTYPE_FP16) return FMHA_ERR_UNSUPPORTED;
+  if (!(A.softmax_scale >= 0.0f) || std::isinf(A.softmax_scale)) return FMHA_ERR_INVALID_ARG;
+  if (A.total_q == 0 || A.batch == 0) return FMHA_OK;
+  if ((st = check_rows(A.q, A.q_stride, hq, d)) != FMHA_OK ||
+      (st = check_rows(A.o, A.o_stride, hq, d)) != FMHA_OK)
     return st;
-  if (total_kv > 0 && ((st = check_rows(K, k_stride, num_heads_kv, head_dim)) != FMHA_OK ||
-                       (st = check_rows(V, v_stride, num_heads_kv, head_dim)) != FMHA_OK))
+  const bool keys = A.total_kv > 0;
+  if (keys && ((st = check_rows(A.k, A.k_stride, hkv, d)) != FMHA_OK ||
+               (st = check_rows(A.v, A.v_stride, hkv, d)) != FMHA_OK))
     return st;
-  if (!cu_seqlens_q) return FMHA_ERR_INVALID_ARG;
-  if (!cu_seqlens_kv && total_kv != total_q) return FMHA_ERR_INVALID_ARG;
-  if ((reinterpret_cast<uintptr_t>(LSE) | reinterpret_cast<uintptr_t>(cu_seqlens_q) |
-       reinterpret_cast<uintptr_t>(cu_seqlens_kv)) & 3u)
+  if (!A.cu_seqlens_q) return FMHA_ERR_INVALID_ARG;
+  if (!A.cu_seqlens_kv && A.total_kv != A.total_q) return FMHA_ERR_INVALID_ARG;
+  if ((reinterpret_cast<uintptr_t>(A.lse) | reinterpret_cast<uintptr_t>(A.cu_seqlens_q) |
+       reinterpret_cast<uintptr_t>(A.cu_seqlens_kv)) & 3u)
     return FMHA_ERR_MISALIGNED;
   ServingDevice dev;
   if ((st = serving_device(&dev)) != FMHA_OK) return st;
   PromptParams P;
   std::memset(&P, 0, sizeof(P));
-  P.q = static_cast<const uint16_t*>(Q);
-  P.k = static_cast<const uint16_t*>(K);
-  P.v = static_cast<const uint16_t*>(V);
-  P.o = static_cast<uint16_t*>(O);
-  P.lse = LSE;
-  P.cu_q = cu_seqlens_q;
-  P.cu_kv = cu_seqlens_kv ? cu_seqlens_kv : cu_seqlens_q;
-  P.total_q = total_q;
-  P.total_kv = total_kv;
-  P.batch = batch;
-  P.hq = num_heads_q;
-  P.hkv = num_heads_kv;
-  P.q_stride = q_stride;
-  P.k_stride = k_stride;
-  P.v_stride = v_stride;
-  P.o_stride = o_stride;
+  P.q = static_cast<const uint16_t*>(A.q);
+  P.k = static_cast<const uint16_t*>(A.k);
+  P.v = static_cast<const uint16_t*>(A.v);
+  P.o = static_cast<uint16_t*>(A.o);
+  P.lse = A.lse;
+  P.cu_q = A.cu_seqlens_q;
+  P.cu_kv = A.cu_seqlens_kv ? A.cu_seqlens_kv : A.cu_seqlens_q;
+  P.total_q = A.total_q;
+  P.total_kv = A.total_kv;
+  P.batch = A.batch;
+  P.hq = hq;
+  P.hkv = hkv;
+  P.q_stride = A.q_stride;
+  P.k_stride = A.k_stride;
+  P.v_stride = A.v_stride;
+  P.o_stride = A.o_stride;
   const double scale =
-      softmax_scale > 0.0f ? (double)softmax_scale : 1.0 / std::sqrt((double)head_dim);
+      A.softmax_scale > 0.0f ? (double)A.softmax_scale : 1.0 / std::sqrt((double)d);
   P.scale_log2 = (float)(1.4426950408889634 * scale);
-  P.causal = causal != 0;
-  P.o_bf16 = o_dtype == FMHA_DTYPE_BF16;
+  P.causal = A.causal != 0;
+  P.o_bf16 = A.o_dtype == FMHA_DTYPE_BF16;
   P.err = dev.err;
-  const bool bf16 = dtype == FMHA_DTYPE_BF16;
-  const int g = num_heads_q / num_heads_kv;
+  const bool bf16 = A.dtype == FMHA_DTYPE_BF16;
+  const int g = hq / hkv;
   while (P.pack_log2 < 7 && (g >> P.pack_log2) % 2 == 0) ++P.pack_log2;
   const int pack = 1 << P.pack_log2;
-  // Without keys no map is used; K's then describes Q.
-  const bool keys = total_kv > 0;
-  if (!encode(&P.map_q, bf16, Q, head_dim, num_heads_q, total_q, q_stride, pack, kTileRows / pack) ||
-      !encode(&P.map_k, bf16, keys ? K : Q, head_dim, keys ? num_heads_kv : num_heads_q,
-              keys ? total_kv : total_q, keys ? k_stride : q_stride, 1, kKeys) ||
-      !encode(&P.map_v, bf16, keys ? V : Q, head_dim, keys ? num_heads_kv : num_heads_q,
-              keys ? total_kv : total_q, keys ? v_stride : q_stride, 1, kKeys))
+  // Without keys no key is loaded; their maps then describe Q.
+  if (!encode(&P.map_q, bf16, A.q, d, hq, A.total_q, A.q_stride, pack, kTileRows / pack) ||
+      !encode(&P.map_k, bf16, keys ? A.k : A.q, d, keys ? hkv : hq,
+              keys ? A.total_kv : A.total_q, keys ? A.k_stride : A.q_stride, 1, kKeys) ||
+      !encode(&P.map_v, bf16, keys ? A.v : A.q, d, keys ? hkv : hq,
+              keys ? A.total_kv : A.total_q, keys ? A.v_stride : A.q_stride, 1, kKeys))
     return FMHA_ERR_CUDA;
   const bool split = bf16 && !P.o_bf16;
-  const PromptFn fn = head_dim == 128 ? prompt_fn<128>(bf16, split) : prompt_fn<256>(bf16, split);
-  const int smem = head_dim == 128 ? PromptShape<128>::kSmem : PromptShape<256>::kSmem;
-  const int threads = head_dim == 128 ? PromptShape<128>::kThreads : PromptShape<256>::kThreads;
+  const PromptFn fn = d == 128 ? prompt_fn<128>(bf16, split) : prompt_fn<256>(bf16, split);
+  const int smem = d == 128 ? PromptShape<128>::kSmem : PromptShape<256>::kSmem;
+  const int threads = d == 128 ? PromptShape<128>::kThreads : PromptShape<256>::kThreads;
   if ((st = ensure_smem(reinterpret_cast<const void*>(fn), smem)) != FMHA_OK) return st;
   // No more work than this, whatever the lengths: each sequence has one part that is not full.
-  const int tokens = (head_dim == 128 ? 2 : 1) * kTileRows / pack;
-  const int64_t parts = ((int64_t)batch + total_q / tokens) * (num_heads_q / pack);
+  const int tokens = (d == 128 ? 2 : 1) * kTileRows / pack;
+  const int64_t parts = ((int64_t)A.batch + A.total_q / tokens) * (hq / pack);
   if (parts > 0x7fffffff) return FMHA_ERR_UNSUPPORTED;
   return launch_serving(fn, dim3((unsigned)parts), threads, smem,
                         reinterpret_cast<cudaStream_t>(stream), P);

@@ -281,70 +281,69 @@ AppendFn append_fn(bool bf16, bool f8, bool inter, int d) {
 
 using namespace fmha;
 
-extern "C" fmha_status_t fmha_rope_append(
-    const void* Q, const void* K, const void* V, void* Q_out, void* K_out,
-    const fmha_paged_cache_t* cache, const int32_t* cu_seqlens_q, const float* cos_table,
-    const float* sin_table, int total_tokens, int batch, int num_heads_q, int num_heads_kv,
-    int head_dim, int64_t q_stride, int64_t k_stride, int64_t v_stride, int64_t q_out_stride,
-    int64_t k_out_stride, int rotary_dim, int max_position, int interleaved, int dtype,
-    fmha_stream_t stream) {
-  if (total_tokens < 0 || batch < 0 || rotary_dim < 0) return FMHA_ERR_INVALID_ARG;
-  fmha_status_t st = check_heads(num_heads_q, num_heads_kv, head_dim);
+extern "C" fmha_status_t fmha_rope_append(const fmha_rope_append_args_t* args,
+                                          fmha_stream_t stream) {
+  if (!args) return FMHA_ERR_INVALID_ARG;
+  const fmha_rope_append_args_t& A = *args;
+  if (A.total_tokens < 0 || A.batch < 0 || A.rotary_dim < 0) return FMHA_ERR_INVALID_ARG;
+  fmha_status_t st = check_heads(A.num_heads_q, A.num_heads_kv, A.head_dim);
   if (st != FMHA_OK) return st;
-  if (dtype != FMHA_DTYPE_BF16 && dtype != FMHA_DTYPE_FP16) return FMHA_ERR_UNSUPPORTED;
-  if (rotary_dim % 16 != 0 || rotary_dim > head_dim) return FMHA_ERR_UNSUPPORTED;
-  if (!cu_seqlens_q && total_tokens != batch) return FMHA_ERR_INVALID_ARG;
-  if (total_tokens == 0 || batch == 0) return FMHA_OK;
-  if ((st = check_rows(Q, q_stride, num_heads_q, head_dim)) != FMHA_OK ||
-      (st = check_rows(K, k_stride, num_heads_kv, head_dim)) != FMHA_OK ||
-      (st = check_rows(V, v_stride, num_heads_kv, head_dim)) != FMHA_OK ||
-      (st = check_rows(Q_out, q_out_stride, num_heads_q, head_dim)) != FMHA_OK ||
-      (K_out && (st = check_rows(K_out, k_out_stride, num_heads_kv, head_dim)) != FMHA_OK))
+  if (A.dtype != FMHA_DTYPE_BF16 && A.dtype != FMHA_DTYPE_FP16) return FMHA_ERR_UNSUPPORTED;
+  if (A.rotary_dim % 16 != 0 || A.rotary_dim > A.head_dim) return FMHA_ERR_UNSUPPORTED;
+  if (!A.cu_seqlens_q && A.total_tokens != A.batch) return FMHA_ERR_INVALID_ARG;
+  if (A.total_tokens == 0 || A.batch == 0) return FMHA_OK;
+  const int hq = A.num_heads_q, hkv = A.num_heads_kv, d = A.head_dim;
+  if ((st = check_rows(A.q, A.q_stride, hq, d)) != FMHA_OK ||
+      (st = check_rows(A.k, A.k_stride, hkv, d)) != FMHA_OK ||
+      (st = check_rows(A.v, A.v_stride, hkv, d)) != FMHA_OK ||
+      (st = check_rows(A.q_out, A.q_out_stride, hq, d)) != FMHA_OK ||
+      (A.k_out && (st = check_rows(A.k_out, A.k_out_stride, hkv, d)) != FMHA_OK))
     return st;
-  if (rotary_dim > 0) {
-    if (!cos_table || !sin_table || max_position <= 0) return FMHA_ERR_INVALID_ARG;
-    if (!aligned16(cos_table) || !aligned16(sin_table)) return FMHA_ERR_MISALIGNED;
+  if (A.rotary_dim > 0) {
+    if (!A.cos_table || !A.sin_table || A.max_position <= 0) return FMHA_ERR_INVALID_ARG;
+    if (!aligned16(A.cos_table) || !aligned16(A.sin_table)) return FMHA_ERR_MISALIGNED;
   }
-  if (reinterpret_cast<uintptr_t>(cu_seqlens_q) & 3u) return FMHA_ERR_MISALIGNED;
+  if (reinterpret_cast<uintptr_t>(A.cu_seqlens_q) & 3u) return FMHA_ERR_MISALIGNED;
   // In place only row upon row: another stride would write rows still to be read.
-  if ((Q_out == Q && q_out_stride != q_stride) || (K_out && K_out == K && k_out_stride != k_stride))
+  if ((A.q_out == A.q && A.q_out_stride != A.q_stride) ||
+      (A.k_out && A.k_out == A.k && A.k_out_stride != A.k_stride))
     return FMHA_ERR_INVALID_ARG;
   AppendParams P;
   std::memset(&P, 0, sizeof(P));
-  if ((st = check_cache(cache, num_heads_kv, head_dim, dtype, &P.cache)) != FMHA_OK) return st;
+  if ((st = check_cache(A.cache, hkv, d, A.dtype, &P.cache)) != FMHA_OK) return st;
   ServingDevice dev;
   if ((st = serving_device(&dev)) != FMHA_OK) return st;
-  P.q = static_cast<const uint16_t*>(Q);
-  P.k = static_cast<const uint16_t*>(K);
-  P.v = static_cast<const uint16_t*>(V);
-  P.q_out = static_cast<uint16_t*>(Q_out);
-  P.k_out = static_cast<uint16_t*>(K_out);
-  P.cu = cu_seqlens_q;
-  P.cos_table = cos_table;
-  P.sin_table = sin_table;
-  P.total_tokens = total_tokens;
-  P.batch = batch;
-  P.hq = num_heads_q;
-  P.hkv = num_heads_kv;
-  P.q_stride = q_stride;
-  P.k_stride = k_stride;
-  P.v_stride = v_stride;
-  P.q_out_stride = q_out_stride;
-  P.k_out_stride = k_out_stride;
-  P.rot = rotary_dim;
-  P.max_position = max_position;
+  P.q = static_cast<const uint16_t*>(A.q);
+  P.k = static_cast<const uint16_t*>(A.k);
+  P.v = static_cast<const uint16_t*>(A.v);
+  P.q_out = static_cast<uint16_t*>(A.q_out);
+  P.k_out = static_cast<uint16_t*>(A.k_out);
+  P.cu = A.cu_seqlens_q;
+  P.cos_table = A.cos_table;
+  P.sin_table = A.sin_table;
+  P.total_tokens = A.total_tokens;
+  P.batch = A.batch;
+  P.hq = hq;
+  P.hkv = hkv;
+  P.q_stride = A.q_stride;
+  P.k_stride = A.k_stride;
+  P.v_stride = A.v_stride;
+  P.q_out_stride = A.q_out_stride;
+  P.k_out_stride = A.k_out_stride;
+  P.rot = A.rotary_dim;
+  P.max_position = A.max_position;
   P.err = dev.err;
   // A block per token while they fit side by side; with few tokens the heads
   // of each are dealt to several blocks.
-  const int slots = kAppendThreads / (head_dim / 16);
-  const int heads = num_heads_q + 2 * num_heads_kv;
+  const int slots = kAppendThreads / (d / 16);
+  const int heads = hq + 2 * hkv;
   const int resident = dev.sms * 6;
-  const int gx = total_tokens < resident ? total_tokens : resident;
+  const int gx = A.total_tokens < resident ? A.total_tokens : resident;
   int gy = 1;
   const int most = (heads + slots - 1) / slots;
   while (gy < most && gx * gy * 2 <= resident) ++gy;
-  return launch_serving(append_fn(dtype == FMHA_DTYPE_BF16, P.cache.dtype == FMHA_DTYPE_E4M3,
-                                  interleaved != 0, head_dim),
+  return launch_serving(append_fn(A.dtype == FMHA_DTYPE_BF16, P.cache.dtype == FMHA_DTYPE_E4M3,
+                                  A.interleaved != 0, d),
                         dim3(gx, gy), kAppendThreads, 0, reinterpret_cast<cudaStream_t>(stream),
                         P);
 }

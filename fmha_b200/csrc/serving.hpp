@@ -52,10 +52,9 @@ inline fmha_status_t check_rows(const void* p, int64_t stride, int64_t heads, in
 
 // The cache, for sequences whose Q has type `dtype`. Strides along axes of
 // one element are put to what they would be in a dense page.
-inline fmha_status_t check_cache(const fmha_paged_cache_t* in, int hkv, int d, int dtype,
+inline fmha_status_t check_cache(const fmha_paged_cache_t& in, int hkv, int d, int dtype,
                                  fmha_paged_cache_t* out) {
-  if (!in) return FMHA_ERR_INVALID_ARG;
-  fmha_paged_cache_t c = *in;
+  fmha_paged_cache_t c = in;
   if (!c.k || !c.v || !c.block_table || !c.seqlens_kv) return FMHA_ERR_INVALID_ARG;
   if (c.num_pages <= 0 || c.page_size <= 0 || c.max_pages <= 0) return FMHA_ERR_INVALID_ARG;
   if (c.dtype != dtype && c.dtype != FMHA_DTYPE_E4M3) return FMHA_ERR_UNSUPPORTED;

@@ -167,6 +167,7 @@ fmha_status_t fmha_forward_noalloc(const void* Q, const void* K, const void* V,
  * the reference's cache holds at most 16 dense rows.
  *
  * Conventions beyond the ones above:
+ *  - the arguments come in a struct, which the call only reads;
  *  - head_dim is 128 or 256; any num_heads_q that is a multiple of
  *    num_heads_kv;
  *  - `dtype` names the type of Q, K and V (bf16 or fp16), `o_dtype` that of O
@@ -237,19 +238,40 @@ typedef struct fmha_paged_cache {
  * packed, for fmha_prompt; may be K itself). Rows behind the last sequence
  * are left as they were. Two new tokens must not map to one cache row.
  */
-fmha_status_t fmha_rope_append(const void* Q, const void* K, const void* V, void* Q_out,
-                               void* K_out, const fmha_paged_cache_t* cache,
-                               const int32_t* cu_seqlens_q, const float* cos_table,
-                               const float* sin_table, int total_tokens, int batch,
-                               int num_heads_q, int num_heads_kv, int head_dim,
-                               int64_t q_stride, int64_t k_stride, int64_t v_stride,
-                               int64_t q_out_stride, int64_t k_out_stride, int rotary_dim,
-                               int max_position, int interleaved, int dtype,
-                               fmha_stream_t stream);
+typedef struct fmha_rope_append_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  void* k_out;                 /* or null */
+  const int32_t* cu_seqlens_q; /* or null */
+  const float* cos_table;
+  const float* sin_table;
+  int64_t q_stride;
+  int64_t k_stride;
+  int64_t v_stride;
+  int64_t q_out_stride;
+  int64_t k_out_stride;
+  fmha_paged_cache_t cache;
+  int32_t total_tokens;
+  int32_t batch;
+  int32_t num_heads_q;
+  int32_t num_heads_kv;
+  int32_t head_dim;
+  int32_t rotary_dim;
+  int32_t max_position;
+  int32_t interleaved;
+  int32_t dtype;
+} fmha_rope_append_args_t;
 
-/* Bytes of device scratch that fmha_paged_decode needs for these heads (the
- * same for every batch and length); -1 for sizes it does not support. */
-int64_t fmha_paged_decode_workspace(int num_heads_q, int num_heads_kv, int head_dim);
+fmha_status_t fmha_rope_append(const fmha_rope_append_args_t* args, fmha_stream_t stream);
+
+/* Bytes of device scratch that fmha_paged_decode needs for these heads when
+ * the block table has room for max_tokens (max_pages * page_size) tokens of a
+ * sequence: the same for every batch, and 0 for short tables, whose sequences
+ * are not split. -1 for sizes it does not support. */
+int64_t fmha_paged_decode_workspace(int num_heads_q, int num_heads_kv, int head_dim,
+                                    int64_t max_tokens);
 
 /*
  * fmha_paged_decode -- attention of one new token per sequence over the
@@ -258,16 +280,30 @@ int64_t fmha_paged_decode_workspace(int num_heads_q, int num_heads_kv, int head_
  *   Q [batch, num_heads_q, head_dim], O the same in o_dtype;
  *   LSE [batch, num_heads_q] fp32 or null: the natural logarithm of the sum
  *   of exp(scaled score).
- * workspace: at least fmha_paged_decode_workspace(...) bytes, 16-byte
- * aligned, overwritten; calls that may run at the same time (two streams, two
+ * workspace: at least fmha_paged_decode_workspace(...) bytes (null if that is
+ * 0), 16-byte aligned, overwritten; calls that may run at the same time (two streams, two
  * captured graphs) need one each. It holds nothing between calls. The launch
  * depends on no length, so a captured call may be replayed as sequences grow.
  */
-fmha_status_t fmha_paged_decode(const void* Q, const fmha_paged_cache_t* cache, void* O,
-                                float* LSE, int batch, int num_heads_q, int num_heads_kv,
-                                int head_dim, int64_t q_stride, int64_t o_stride,
-                                float softmax_scale, int dtype, int o_dtype, void* workspace,
-                                int64_t workspace_bytes, fmha_stream_t stream);
+typedef struct fmha_paged_decode_args {
+  const void* q;
+  void* o;
+  float* lse; /* or null */
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t q_stride;
+  int64_t o_stride;
+  fmha_paged_cache_t cache;
+  int32_t batch;
+  int32_t num_heads_q;
+  int32_t num_heads_kv;
+  int32_t head_dim;
+  int32_t dtype;
+  int32_t o_dtype;
+  float softmax_scale;
+} fmha_paged_decode_args_t;
+
+fmha_status_t fmha_paged_decode(const fmha_paged_decode_args_t* args, fmha_stream_t stream);
 
 /*
  * fmha_prompt -- attention over packed prompts of different lengths:
@@ -280,12 +316,31 @@ fmha_status_t fmha_paged_decode(const void* Q, const fmha_paged_cache_t* cache, 
  * query i of nq sees keys j <= i + (nk - nq): the last query sees every key.
  * Rows behind the last sequence are left as they were.
  */
-fmha_status_t fmha_prompt(const void* Q, const void* K, const void* V, void* O, float* LSE,
-                          const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_kv,
-                          int total_q, int total_kv, int batch, int num_heads_q,
-                          int num_heads_kv, int head_dim, int64_t q_stride, int64_t k_stride,
-                          int64_t v_stride, int64_t o_stride, float softmax_scale, int causal,
-                          int dtype, int o_dtype, fmha_stream_t stream);
+typedef struct fmha_prompt_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  float* lse; /* or null */
+  const int32_t* cu_seqlens_q;
+  const int32_t* cu_seqlens_kv; /* or null */
+  int64_t q_stride;
+  int64_t k_stride;
+  int64_t v_stride;
+  int64_t o_stride;
+  int32_t total_q;
+  int32_t total_kv;
+  int32_t batch;
+  int32_t num_heads_q;
+  int32_t num_heads_kv;
+  int32_t head_dim;
+  int32_t causal;
+  int32_t dtype;
+  int32_t o_dtype;
+  float softmax_scale;
+} fmha_prompt_args_t;
+
+fmha_status_t fmha_prompt(const fmha_prompt_args_t* args, fmha_stream_t stream);
 
 /* Human-readable name of a status code (static storage). Reference
  * counterpart: the HIP_CHECK error text (fmha_host.cpp:26-35). */

@@ -419,7 +419,7 @@ def test_decode_streams_graphs_and_workspace(cuda):
     with torch.cuda.stream(side):
         fmha_b200.fmha_paged_decode(*args)
     torch.cuda.synchronize()
-    need = fmha_b200.fmha_paged_decode_workspace(hq, hkv, d)
+    need = fmha_b200.fmha_paged_decode_workspace(hq, hkv, d, table.shape[1] * size)
     graphs, outs = [], []
     for own in (False, True):
         out = torch.zeros_like(want)
