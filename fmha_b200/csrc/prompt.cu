@@ -18,9 +18,15 @@
 //
 // Warps: 4 per tile for the softmax (one thread per row: a row's maximum and
 // sum need no shuffles), one to issue TMA loads (a ring of 32 KB stages: 128
-// keys x 128 columns of K or V), one to issue the MMAs. S (128 fp32 columns)
-// and P (64 columns of 16-bit pairs, over S) stay in tensor memory; P is the
-// A operand of P.V from there.
+// keys x 128 columns of K or V), one to issue the MMAs, one that plans, one
+// that clears V rows. S (128 fp32 columns) and P (64 columns of 16-bit pairs, over S) stay in tensor
+// memory; P is the A operand of P.V from there.
+//
+// One CTA per SM stays and takes piece after piece: its own first, then, by
+// cluster launch control, those of blocks that have not started. The planning
+// warp finds each piece's sequence one ahead; Q and the first keys of the next
+// piece are loaded, and its first scores computed, while the outputs of the
+// last are written.
 //
 // Precision: P is rounded to the operands' type, except that bf16 operands
 // with an fp16 result take P as two bf16 parts and a second P.V product, so
@@ -76,7 +82,9 @@ struct PromptShape {
   static constexpr int kTiles = D == 128 ? 2 : 1;    // query tiles of a CTA
   static constexpr int kHalves = D / 128;            // 128-column parts of a head
   static constexpr int kSoftWarps = 4 * kTiles;
-  static constexpr int kThreads = 32 * (kSoftWarps + 2);
+  static constexpr int kTmaWarp = kSoftWarps, kMmaWarp = kTmaWarp + 1, kPlanWarp = kMmaWarp + 1,
+                       kTrimWarp = kPlanWarp + 1;
+  static constexpr int kThreads = 32 * (kSoftWarps + 4);
   static constexpr int kQBytes = 2 * kStageBytes;    // either two tiles or two halves
   static constexpr int kStages = 5;
   static constexpr int kSmem = kQBytes + kStages * kStageBytes + 1024;  // aligned to 1024 inside
@@ -88,15 +96,17 @@ struct Work {
   int tok0;            // its first token here
   int head0;           // first of the PACK heads
   int kvh;
+  int n0, n1;          // key blocks of its tiles; -1: no row in that tile
+  int last;            // nothing, and nothing follows
 };
 
-// The CTA's sequence and tokens: tiles of one sequence go from its end to its
+// Piece `index` of the work: tiles of one sequence go from its end to its
 // start, the longest first. False behind the last tile. One warp.
-__device__ bool find_work(const PromptParams& P, int tokens, Work* out) {
+__device__ bool find_work(const PromptParams& P, int index, int tokens, Work* out) {
   const int lane = threadIdx.x & 31;
   const int groups = P.hq >> P.pack_log2;
-  const int group = blockIdx.x % groups;
-  int at = blockIdx.x / groups;
+  const int group = index % groups;
+  int at = index / groups;
   for (int b0 = 0; b0 < P.batch; b0 += 32) {
     const int b = b0 + lane;
     int64_t len = 0;
@@ -151,13 +161,13 @@ __device__ __forceinline__ int tile_blocks(const PromptParams& P, const Work& w,
 // the row's own `seen` keys, divided by l. For rows that met a NaN or an
 // infinity behind their last key in the tensor cores.
 template <int D, bool BF16>
-__device__ __noinline__ void row_again(const PromptParams& P, const Work& w, int tok, int head,
-                                       int seen, float neg, float l) {
+__device__ __noinline__ void row_again(const PromptParams& P, int64_t q_row, int64_t k_row, int head,
+                                       int kvh, int seen, float neg, float l) {
   constexpr int kMine = D / 32;  // columns of a lane
   const int lane = threadIdx.x & 31;
-  const uint16_t* const q = P.q + (int64_t)(w.q0 + tok) * P.q_stride + (int64_t)head * D;
-  const uint16_t* const k = P.k + (int64_t)w.k0 * P.k_stride + (int64_t)w.kvh * D;
-  const uint16_t* const v = P.v + (int64_t)w.k0 * P.v_stride + (int64_t)w.kvh * D + kMine * lane;
+  const uint16_t* const q = P.q + q_row * P.q_stride + (int64_t)head * D;
+  const uint16_t* const k = P.k + k_row * P.k_stride + (int64_t)kvh * D;
+  const uint16_t* const v = P.v + k_row * P.v_stride + (int64_t)kvh * D + kMine * lane;
   float o[kMine] = {};
   for (int j0 = 0; j0 < seen; j0 += 32) {
     float s = 0.0f;
@@ -183,7 +193,7 @@ __device__ __noinline__ void row_again(const PromptParams& P, const Work& w, int
     }
   }
   uint32_t* const out = reinterpret_cast<uint32_t*>(
-      P.o + (int64_t)(w.q0 + tok) * P.o_stride + (int64_t)head * D + kMine * lane);
+      P.o + q_row * P.o_stride + (int64_t)head * D + kMine * lane);
 #pragma unroll
   for (int i = 0; i < kMine / 2; ++i) {
     const float a = o[2 * i] / l, b = o[2 * i + 1] / l;
@@ -198,44 +208,47 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
   constexpr int kTiles = S::kTiles, kHalves = S::kHalves, kStages = S::kStages;
   // Weights in fp16 carry 2^7, so that small ones keep clear of its short exponent.
   constexpr float kShift = BF16 ? 0.0f : 7.0f;
+  // Barriers: ring stages filled and free; Q in and free; scores ready and
+  // weights ready (per tile, or per score buffer); output done and drained
+  // (per tile); a piece of work posted and read; an answer of the scheduler.
+  enum {
+    kFull = 0,
+    kEmpty = kFull + S::kStages,
+    kQFull = kEmpty + S::kStages,
+    kQFree,
+    kSFull,
+    kPFull = kSFull + 2,
+    kODone = kPFull + 2,
+    kOFree = kODone + 2,
+    kWorkFull = kOFree + 2,
+    kWorkFree = kWorkFull + 2,
+    kAnswer = kWorkFree + 2,
+    kTrimGo,
+    kTrimmed,
+    kDrain,
+    kBars
+  };
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * kStages + 8];
+  __shared__ __align__(8) uint64_t bars[kBars];
+  __shared__ __align__(16) uint4 answer;
   __shared__ uint32_t tmem_slot;
-  __shared__ Work work;
-  __shared__ int have_work;
+  __shared__ Work work[2];
+  __shared__ uint2 trim_at;  // the stage with rows to clear, and how many to keep
   __shared__ volatile int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   allow_dependent_launch();
   grid_dependency_wait();
 
-  if (warp == 0) {
-    Work w;
-    const bool found = find_work(P, kTiles * (kTileRows >> P.pack_log2), &w);
-    if (lane == 0) {
-      if (found) work = w;
-      have_work = found;
-      abort_flag = 0;
-    }
-  }
-  __syncthreads();
-  if (!have_work) return;
-
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](int i) { return bar0 + 8 * i; };
-  constexpr int kFull = 0, kEmpty = kStages, kQFull = 2 * kStages, kSFull = kQFull + 1,
-                kPFull = kSFull + 2, kODone = kPFull + 2, kDrain = kODone + 2;
-  if (warp == S::kSoftWarps + 1) {
+  if (warp == S::kMmaWarp) {
     if (lane == 0) {
-      for (int i = 0; i < kStages; ++i) {
-        mbar_init(bar(kFull + i), 1);
-        mbar_init(bar(kEmpty + i), 1);
-      }
-      mbar_init(bar(kQFull), 1);
-      mbar_init(bar(kDrain), 1);
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(bar(kSFull + i), 1);
-        mbar_init(bar(kPFull + i), 4);
-        mbar_init(bar(kODone + i), 1);
+      abort_flag = 0;
+      for (int i = 0; i < kBars; ++i) {
+        int count = 1;
+        if ((i >= kPFull && i < kPFull + 2) || (i >= kOFree && i < kOFree + 2)) count = 4;
+        if (i >= kWorkFree && i < kWorkFree + 2) count = S::kSoftWarps + 3;  // TMA, MMA, trim
+        mbar_init(bar(i), count);
       }
       fence_mbar_init();
       fence_async_shared();
@@ -247,313 +260,157 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = tmem_slot;
-  const Work w = work;
   const uint32_t sq = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t ring = sq + S::kQBytes;
-  const int n0 = tile_blocks(P, w, 0);
-  const int n1 = kTiles == 2 ? tile_blocks(P, w, 1) : -1;
-  const int blocks = max(n0, n1);
+  const int tokens = kTileRows >> P.pack_log2;  // of a tile
   auto wait = [&](int b, uint32_t parity) {  // one thread
     return mbar_wait(bar(b), parity, &abort_flag, P.err, kWaitTimeoutNs, kSitePromptWait);
   };
   auto wait_warp = [&](int b, uint32_t parity) {  // a whole warp, of one mind
     return __all_sync(kFullMask, wait(b, parity)) != 0;
   };
-
-  if (warp == S::kSoftWarps) {
-    // ---------------------------------------------------------- TMA loads
-    if (lane == 0 && blocks > 0) {
-      const int tokens = kTileRows >> P.pack_log2;
-      mbar_arrive_expect_tx(bar(kQFull), (kTiles == 2 && n1 < 0 ? 1 : 2) * kStageBytes);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (kTiles == 2 && i == 1 && n1 < 0) break;
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          tma_load_3d(sq + i * kStageBytes + c * kBlockBytes, &P.map_q,
-                      (kTiles == 2 ? 0 : 128 * i) + 64 * c, w.head0,
-                      w.q0 + w.tok0 + (kTiles == 2 ? i * tokens : 0), bar(kQFull));
-      }
-      int slot = 0, use = 0;  // loads go in the order the MMA warp takes them
-      bool ok = true;
-      auto load = [&](const CUtensorMap* map, int j, int h) {
-        if (!ok) return;
-        if (use > 0 && !wait(kEmpty + slot, (use - 1) & 1)) {
-          ok = false;
-          return;
-        }
-        mbar_arrive_expect_tx(bar(kFull + slot), kStageBytes);
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          tma_load_3d(ring + slot * kStageBytes + c * kBlockBytes, map, 128 * h + 64 * c, w.kvh,
-                      w.k0 + j * kKeys, bar(kFull + slot));
-        if (++slot == kStages) {
-          slot = 0;
-          ++use;
-        }
-      };
-      for (int h = 0; h < kHalves; ++h) load(&P.map_k, 0, h);
-      for (int j = 0; j < blocks && ok; ++j) {
-        if (kTiles == 2) {
-          load(&P.map_v, j, 0);
-          if (j + 1 < blocks) load(&P.map_k, j + 1, 0);
-        } else {
-          if (j + 1 < blocks)
-            for (int h = 0; h < kHalves; ++h) load(&P.map_k, j + 1, h);
-          for (int h = 0; h < kHalves; ++h) load(&P.map_v, j, h);
-        }
-      }
-      if (!ok) {
-        // Given up: let this CTA's copies land before its shared memory goes.
-        const uint64_t t0 = globaltimer_ns();
-        for (int i = 0; i < kStages; ++i) {
-          const int uses = use + (i < slot ? 1 : 0);
-          if (uses == 0) continue;
-          while (!mbar_try_wait(bar(kFull + i), (uses - 1) & 1) &&
-                 globaltimer_ns() - t0 < kStallTimeoutNs) {
-          }
-        }
-      }
-    }
-  } else if (warp == S::kSoftWarps + 1) {
-    // ---------------------------------------------------------- MMAs
-    constexpr uint32_t kIdQK = umma_idesc(BF16, 128, false);
-    constexpr uint32_t kIdPV = umma_idesc(BF16, 128, true);
-    bool ok = blocks > 0 && wait_warp(kQFull, 0);
-    int slot = 0, use = 0;
-    auto take = [&]() {  // waits for the next stage; its address
-      ok = ok && wait_warp(kFull + slot, use & 1);
-      return ring + slot * kStageBytes;
-    };
-    auto done = [&]() {  // frees it once the MMAs issued so far are through
-      if (lane == 0) umma_commit(bar(kEmpty + slot));
-      if (++slot == kStages) {
-        slot = 0;
-        ++use;
-      }
-    };
-    // S = Q K^T over one 128-column part.
-    auto qk = [&](uint32_t s_col, uint32_t q, uint32_t k, bool first) {
-      if (lane != 0) return;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t off = (i >> 2) * kBlockBytes + (i & 3) * 32;
-        umma_ss(tmem + s_col, umma_desc(q + off, 16, 1024), umma_desc(k + off, 16, 1024), kIdQK,
-                !(first && i == 0));
-      }
-    };
-    // O += P V over one 128-column part.
-    auto pv = [&](uint32_t o_col, uint32_t p_col, uint32_t v, bool first) {
-      if (lane != 0) return;
-#pragma unroll
-      for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          umma_ts(tmem + o_col, tmem + p_col + part * 64 + i * 8,
-                  umma_desc(v + i * 2048, kBlockBytes, 1024), kIdPV, !(first && part == 0 && i == 0));
-    };
-    // V rows behind the sequence's end, if any, become zeros.
-    auto trim = [&](uint32_t v, int j) {
-      const int have = w.nk - j * kKeys;
-      if (have >= kKeys) return;
-      for (int e = lane; e < (kKeys - have) * 16; e += 32) {
-        const uint32_t at = v + (e & 1) * kBlockBytes + (have + (e >> 4)) * 128 + ((e >> 1) & 7) * 16;
-        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
-      }
-      fence_async_shared();
-      __syncwarp();
-    };
-    if constexpr (kTiles == 2) {
-      if (ok) {
-        const uint32_t k = take();
-        if (ok) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if ((i ? n1 : n0) > 0) {
-              qk(128 * i, sq + i * kStageBytes, k, true);
-              if (lane == 0) umma_commit(bar(kSFull + i));
-            }
-          done();
-        }
-      }
-      for (int j = 0; j < blocks && ok; ++j) {
-        const uint32_t v = take();
-        if (!ok) break;
-        const int v_slot = slot;
-        if (++slot == kStages) {
-          slot = 0;
-          ++use;
-        }
-        trim(v, j);
-        uint32_t k = 0;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int n = i ? n1 : n0;
-          if (j < n) {
-            ok = ok && wait_warp(kPFull + i, j & 1);
-            if (!ok) break;
-            tmem_fence_after();
-            pv(S::kColO + 128 * i, 128 * i, v, j == 0);
-            if (lane == 0 && j + 1 == n) umma_commit(bar(kODone + i));
-          }
-          if (i == 1 && lane == 0) umma_commit(bar(kEmpty + v_slot));
-          if (j + 1 < n) {
-            if (k == 0) k = take();
-            if (!ok) break;
-            qk(128 * i, sq + i * kStageBytes, k, true);
-            if (lane == 0) umma_commit(bar(kSFull + i));
-          }
-        }
-        if (ok && j + 1 < blocks) done();
-      }
-    } else {
-      auto scores = [&](int j) {
-        for (int h = 0; h < kHalves && ok; ++h) {
-          const uint32_t k = take();
-          if (!ok) return;
-          qk(128 * (j & 1), sq + h * kStageBytes, k, h == 0);
-          done();
-        }
-        if (lane == 0 && ok) umma_commit(bar(kSFull + (j & 1)));
-      };
-      if (ok) scores(0);
-      for (int j = 0; j < blocks && ok; ++j) {
-        if (j + 1 < blocks) scores(j + 1);
-        ok = ok && wait_warp(kPFull + (j & 1), (j >> 1) & 1);
-        if (!ok) break;
-        tmem_fence_after();
-        for (int h = 0; h < kHalves && ok; ++h) {
-          const uint32_t v = take();
-          if (!ok) break;
-          trim(v, j);
-          pv(S::kColO + 128 * h, 128 * (j & 1), v, j == 0);
-          done();
-        }
-        if (lane == 0 && ok) umma_commit(bar(kODone));
-      }
-    }
-    if (blocks > 0 && !ok && lane == 0) {
-      // Given up: let the MMAs in flight end before their memory goes.
-      umma_commit(bar(kDrain));
-      const uint64_t t0 = globaltimer_ns();
-      while (!mbar_try_wait(bar(kDrain), 0) && globaltimer_ns() - t0 < kStallTimeoutNs) {
-      }
-    }
+  // The next piece of work, by one thread; false at the end or on giving up.
+  int piece = 0;
+  Work w;
+  auto next_work_one = [&]() {
+    const int s = piece & 1;
+    if (!wait(kWorkFull + s, (piece >> 1) & 1)) return false;
+    w = work[s];
+    mbar_arrive(bar(kWorkFree + s));
+    ++piece;
+    return w.last == 0;
+  };
+  auto next_work = [&]() {  // by a whole warp
+    const int s = piece & 1;
+    if (!wait_warp(kWorkFull + s, (piece >> 1) & 1)) return false;
+    w = work[s];
     __syncwarp();
-  } else {
+    if (lane == 0) mbar_arrive(bar(kWorkFree + s));
+    ++piece;
+    return w.last == 0;
+  };
+
+  // At head_dim 128 three warpgroups start with 168 registers a thread; the
+  // softmax warps take 208 and leave the others 88 (2*208 + 88 = 3*168).
+  if (warp < S::kSoftWarps) {
+    if constexpr (kTiles == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---------------------------------------------------------- softmax
     const int tile = warp >> 2;
     const int row = threadIdx.x & 127;
     const uint32_t lanes = tmem + ((uint32_t)(row & ~31) << 16);
-    const int n = tile ? n1 : n0;
-    const int tokens = kTileRows >> P.pack_log2;
-    const int tok_base = w.tok0 + tile * tokens;
-    const int tok = tok_base + (row >> P.pack_log2);
-    const int ahead = w.nk - w.nq;
-    const int seen = P.causal ? max(0, min(w.nk, tok + ahead + 1)) : w.nk;  // keys of this row
-    const int warp_tok = tok_base + ((row & ~31) >> P.pack_log2);
-    const int least = P.causal ? min(w.nk, warp_tok + ahead + 1) : w.nk;  // of the warp's first row
+    const uint32_t o_at = lanes + S::kColO + (kTiles == 2 ? 128 * tile : 0);
     const float sc = P.scale_log2;
-    float m = -INFINITY, l = 0.0f;
+    int block = 0;    // key blocks so far, of this tile
+    int outputs = 0;  // and outputs (head_dim 128)
     bool ok = true;
-    for (int j = 0; j < n; ++j) {
-      const int buf = kTiles == 2 ? tile : j & 1;
-      ok = wait_warp(kSFull + buf, kTiles == 2 ? j & 1 : (j >> 1) & 1);
-      if (!ok) break;
-      tmem_fence_after();
-      const uint32_t s_at = lanes + 128 * buf;
-      uint32_t x[4][32];
+    while (ok && next_work()) {
+      const int n = tile ? w.n1 : w.n0;
+      if (n < 0) continue;
+      const int tok_base = w.tok0 + tile * tokens;
+      const int tok = tok_base + (row >> P.pack_log2);
+      const int ahead = w.nk - w.nq;
+      const int seen = P.causal ? max(0, min(w.nk, tok + ahead + 1)) : w.nk;  // keys of this row
+      const int warp_tok = tok_base + ((row & ~31) >> P.pack_log2);
+      const int least = P.causal ? min(w.nk, warp_tok + ahead + 1) : w.nk;  // of the warp's first row
+      float m = -INFINITY, l = 0.0f;
+      for (int j = 0; j < n; ++j, ++block) {
+        const int buf = kTiles == 2 ? tile : block & 1;
+        ok = wait_warp(kSFull + buf, kTiles == 2 ? block & 1 : (block >> 1) & 1);
+        if (!ok) break;
+        tmem_fence_after();
+        const uint32_t s_at = lanes + 128 * buf;
+        uint32_t x[4][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(x[c], s_at + 32 * c);
-      tmem_wait_ld();
-      if ((j + 1) * kKeys > least) {
-        const int left = seen - j * kKeys;
+        for (int c = 0; c < 4; ++c) tmem_ld32(x[c], s_at + 32 * c);
+        tmem_wait_ld();
+        if ((j + 1) * kKeys > least) {
+          const int left = seen - j * kKeys;
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (32 * c + i >= left) x[c][i] = 0xff800000u;
-      }
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            for (int i = 0; i < 32; ++i)
+              if (32 * c + i >= left) x[c][i] = 0xff800000u;
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
+        for (int i = 0; i < 32; ++i)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], __uint_as_float(x[c][i]));
-      const float now = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
-      if (j == 0) {
-        m = now;
-      } else {
-        const bool rise = (now - m) * sc > kSlack;
-        if (__any_sync(kFullMask, rise)) {
-          // The scores of block j follow P.V of block j-1 (head_dim 128), or of j-2 (256).
-          if (kTiles == 1) {
-            ok = wait_warp(kODone, (j - 1) & 1);
-            if (!ok) break;
-            tmem_fence_after();
-          }
-          float f = 1.0f;
-          if (rise) {
-            f = ex2((m - now) * sc);
-            m = now;
-            l *= f;
-          }
-          __syncwarp();
+          for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], __uint_as_float(x[c][i]));
+        const float now = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+        if (j == 0) {
+          m = now;
+        } else {
+          const bool rise = (now - m) * sc > kSlack;
+          if (__any_sync(kFullMask, rise)) {
+            // The scores of block j follow P.V of block j-1 (head_dim 128), or of j-2 (256).
+            if (kTiles == 1) {
+              ok = wait_warp(kODone, (block - 1) & 1);
+              if (!ok) break;
+              tmem_fence_after();
+            }
+            float f = 1.0f;
+            if (rise) {
+              f = ex2((m - now) * sc);
+              m = now;
+              l *= f;
+            }
+            __syncwarp();
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            const uint32_t at = lanes + S::kColO + (kTiles == 2 ? 128 * tile : 0) + 32 * c;
-            uint32_t y[32];
-            tmem_ld32(y, at);
-            tmem_wait_ld();
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t y[32];
+              tmem_ld32(y, o_at + 32 * c);
+              tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
-            tmem_st32(at, y);
+              for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+              tmem_st32(o_at + 32 * c, y);
+            }
           }
         }
-      }
-      const float neg = m == -INFINITY ? 0.0f : kShift - m * sc;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const float neg = m == -INFINITY ? 0.0f : kShift - m * sc;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 4; ++c) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float p = ex2(fmaf(__uint_as_float(x[c][i]), sc, neg));
-          sum[i & 3] += p;
-          x[c][i] = __float_as_uint(p);
+          for (int i = 0; i < 32; ++i) {
+            const float p = ex2(fmaf(__uint_as_float(x[c][i]), sc, neg));
+            sum[i & 3] += p;
+            x[c][i] = __float_as_uint(p);
+          }
         }
-      }
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t hi[32], lo[SPLIT ? 32 : 1];
+        for (int c = 0; c < 2; ++c) {
+          uint32_t hi[32], lo[SPLIT ? 32 : 1];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float a = __uint_as_float(x[2 * c + (i >> 4)][(2 * i) & 31]);
-          const float b = __uint_as_float(x[2 * c + (i >> 4)][((2 * i) & 31) + 1]);
-          if constexpr (SPLIT)
-            split2<BF16>(a, b, hi[i], lo[i]);
-          else
-            hi[i] = pack2<BF16>(a, b);
+          for (int i = 0; i < 32; ++i) {
+            const float a = __uint_as_float(x[2 * c + (i >> 4)][(2 * i) & 31]);
+            const float b = __uint_as_float(x[2 * c + (i >> 4)][((2 * i) & 31) + 1]);
+            if constexpr (SPLIT)
+              split2<BF16>(a, b, hi[i], lo[i]);
+            else
+              hi[i] = pack2<BF16>(a, b);
+          }
+          tmem_st32(s_at + 32 * c, hi);
+          if constexpr (SPLIT) tmem_st32(s_at + 64 + 32 * c, lo);
         }
-        tmem_st32(s_at + 32 * c, hi);
-        if constexpr (SPLIT) tmem_st32(s_at + 64 + 32 * c, lo);
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kPFull + buf));
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_wait_st();
-      tmem_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kPFull + buf));
-    }
 
-    if (ok && n > 0) {
-      if (kTiles == 2) {
-        ok = wait_warp(kODone + tile, 0);
-      } else {
-        // One phase after the other: the last but one may still be open.
-        if (n > 1) ok = wait_warp(kODone, n & 1);
-        ok = ok && wait_warp(kODone, (n - 1) & 1);
+      if (ok && n > 0) {
+        if (kTiles == 2) {
+          ok = wait_warp(kODone + tile, outputs & 1);
+          ++outputs;
+        } else {
+          // One phase after the other: the last but one may still be open.
+          if (n > 1) ok = wait_warp(kODone, (block - 2) & 1);
+          ok = ok && wait_warp(kODone, (block - 1) & 1);
+        }
+        tmem_fence_after();
       }
-      tmem_fence_after();
-    }
-    if (ok && n >= 0) {
+      if (!ok) break;
       const bool mine = tok < w.nq;
       const int head = w.head0 + (row & ((1 << P.pack_log2) - 1));
       const bool none = seen == 0;
@@ -564,8 +421,13 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
       for (int c = 0; c < D / 32; ++c) {
         uint32_t y[32];
         if (n > 0) {
-          tmem_ld32(y, lanes + S::kColO + (kTiles == 2 ? 128 * tile : 0) + 32 * c);
+          tmem_ld32(y, o_at + 32 * c);
           tmem_wait_ld();
+          if (c + 1 == D / 32) {  // the next output may take its place
+            tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(kOFree + (kTiles == 2 ? tile : 0)));
+          }
         }
         if (mine) {
 #pragma unroll
@@ -592,15 +454,304 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
       while (again) {
         const int r = __ffs(again) - 1;
         again &= again - 1;
-        row_again<D, BF16>(P, w, __shfl_sync(kFullMask, tok, r), __shfl_sync(kFullMask, head, r),
-                           __shfl_sync(kFullMask, seen, r), __shfl_sync(kFullMask, neg, r),
-                           __shfl_sync(kFullMask, l, r));
+        row_again<D, BF16>(P, w.q0 + __shfl_sync(kFullMask, tok, r), w.k0,
+                           __shfl_sync(kFullMask, head, r), w.kvh, __shfl_sync(kFullMask, seen, r),
+                           __shfl_sync(kFullMask, neg, r), __shfl_sync(kFullMask, l, r));
       }
     }
     tmem_fence_before();
+  } else {
+    if constexpr (kTiles == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == S::kPlanWarp) {
+      // ---------------------------------------------------------- work list
+      // This block's own piece first, then those of blocks that have not
+      // started, until there are none.
+      int index = blockIdx.x, asked = 0;
+      bool ok = true;
+      while (ok) {
+        if (lane == 0 && index >= 0) {
+          fence_async_shared();  // the last answer has been read
+          mbar_arrive_expect_tx(bar(kAnswer), 16);
+          clc_try_cancel(smem_u32(&answer), bar(kAnswer));
+        }
+        Work mine;
+        const bool found = index >= 0 && find_work(P, index, kTiles * tokens, &mine);
+        if (found || index < 0) {
+          mine.last = index < 0;
+          if (found) {
+            mine.n0 = tile_blocks(P, mine, 0);
+            mine.n1 = kTiles == 2 ? tile_blocks(P, mine, 1) : -1;
+          }
+          const int s = piece & 1;
+          if (piece >= 2) ok = wait_warp(kWorkFree + s, ((piece >> 1) - 1) & 1);
+          if (ok && lane == 0) {
+            work[s] = mine;
+            mbar_arrive(bar(kWorkFull + s));
+          }
+          ++piece;
+        }
+        if (index < 0) break;
+        // The answer is always waited for, so that it lands while the block is there.
+        const bool got = wait_warp(kAnswer, asked & 1);
+        ok = ok && got;
+        ++asked;
+        if (got) index = clc_granted(smem_u32(&answer));
+        __syncwarp();
+      }
+    } else if (warp == S::kTmaWarp) {
+      // ---------------------------------------------------------- TMA loads
+      int slot = 0, use = 0;  // loads go in the order the MMA warp takes them
+      bool ok = true;
+      auto load = [&](const CUtensorMap* map, int j, int h) {
+        if (!ok) return;
+        if (use > 0 && !wait(kEmpty + slot, (use - 1) & 1)) {
+          ok = false;
+          return;
+        }
+        mbar_arrive_expect_tx(bar(kFull + slot), kStageBytes);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          tma_load_3d(ring + slot * kStageBytes + c * kBlockBytes, map, 128 * h + 64 * c, w.kvh,
+                      w.k0 + j * kKeys, bar(kFull + slot));
+        if (++slot == kStages) {
+          slot = 0;
+          ++use;
+        }
+      };
+      int loaded = 0;  // pieces whose Q was loaded
+      while (__shfl_sync(kFullMask, (int)ok, 0) && next_work()) {
+        const int blocks = max(w.n0, w.n1);
+        if (lane == 0 && blocks > 0) {
+          if (loaded > 0) ok = wait(kQFree, (loaded - 1) & 1);
+          if (ok) {
+            ++loaded;
+            mbar_arrive_expect_tx(bar(kQFull), (kTiles == 2 && w.n1 < 0 ? 1 : 2) * kStageBytes);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if (kTiles == 2 && i == 1 && w.n1 < 0) break;
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+                tma_load_3d(sq + i * kStageBytes + c * kBlockBytes, &P.map_q,
+                            (kTiles == 2 ? 0 : 128 * i) + 64 * c, w.head0,
+                            w.q0 + w.tok0 + (kTiles == 2 ? i * tokens : 0), bar(kQFull));
+            }
+          }
+          for (int h = 0; h < kHalves; ++h) load(&P.map_k, 0, h);
+          for (int j = 0; j < blocks && ok; ++j) {
+            if (kTiles == 2) {
+              load(&P.map_v, j, 0);
+              if (j + 1 < blocks) load(&P.map_k, j + 1, 0);
+            } else {
+              if (j + 1 < blocks)
+                for (int h = 0; h < kHalves; ++h) load(&P.map_k, j + 1, h);
+              for (int h = 0; h < kHalves; ++h) load(&P.map_v, j, h);
+            }
+          }
+        }
+        __syncwarp();
+      }
+      if (lane == 0 && abort_flag) {
+        // Given up: let this CTA's copies land before its shared memory goes.
+        const uint64_t t0 = globaltimer_ns();
+        auto landed = [&](int b, int uses) {
+          while (uses > 0 && !mbar_try_wait(bar(b), (uses - 1) & 1) &&
+                 globaltimer_ns() - t0 < kStallTimeoutNs) {
+          }
+        };
+        for (int i = 0; i < kStages; ++i) landed(kFull + i, use + (i < slot ? 1 : 0));
+        landed(kQFull, loaded);
+      }
+      __syncwarp();
+    } else if (warp == S::kMmaWarp) {
+      // -------------------------------------------------------- MMAs
+      // One thread does it all: waits, issues, commits.
+      if (elect_one()) {
+        constexpr uint32_t kIdQK = umma_idesc(BF16, 128, false);
+        constexpr uint32_t kIdPV = umma_idesc(BF16, 128, true);
+        bool ok = true;
+        int slot = 0, use = 0;
+        int loaded = 0;           // Q tiles taken
+        int trimmed = 0;          // last V blocks cleared
+        int fed0 = 0, fed1 = 0;   // weights taken per tile (head_dim 256: in all)
+        int out0 = 0, out1 = 0;   // outputs begun per tile
+        auto step = [&]() {
+          if (++slot == kStages) {
+            slot = 0;
+            ++use;
+          }
+        };
+        auto take = [&]() {  // waits for the next stage; its address
+          ok = ok && wait(kFull + slot, use & 1);
+          return ring + slot * kStageBytes;
+        };
+        auto done = [&]() {  // frees it once the MMAs issued so far are through
+          umma_commit(bar(kEmpty + slot));
+          step();
+        };
+        // S = Q K^T over one 128-column part.
+        auto qk = [&](uint32_t s_col, uint32_t q, uint32_t k, bool first) {
+          const uint64_t a = umma_desc(q, 16, 1024), b = umma_desc(k, 16, 1024);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t off = ((i >> 2) * kBlockBytes + (i & 3) * 32) >> 4;
+            umma_ss(tmem + s_col, a + off, b + off, kIdQK, !(first && i == 0));
+          }
+        };
+        // O += P V over one 128-column part.
+        auto pv = [&](uint32_t o_col, uint32_t p_col, uint32_t v, bool first) {
+          const uint64_t b = umma_desc(v, kBlockBytes, 1024);
+#pragma unroll
+          for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              umma_ts(tmem + o_col, tmem + p_col + part * 64 + i * 8, b + ((i * 2048) >> 4), kIdPV,
+                      !(first && part == 0 && i == 0));
+        };
+        // V rows behind the sequence's end, if block j has any, are cleared by
+        // the trimming warp.
+        auto trim = [&](int v_slot, int j) {
+          const int have = w.nk - j * kKeys;
+          if (have >= kKeys || !ok) return;
+          trim_at = make_uint2(ring + v_slot * kStageBytes, have);
+          mbar_arrive(bar(kTrimGo));
+          ok = wait(kTrimmed, trimmed & 1);
+          ++trimmed;
+        };
+        // Waits for the next weights of tile (or buffer) i, and before the
+        // first of a piece for the last output of that tile to be drained.
+        auto weights = [&](int b, int& fed, int parity, int drain, int& outs, bool first) {
+          ok = ok && wait(kPFull + b, parity & 1);
+          ++fed;
+          if (first) {
+            if (outs > 0) ok = ok && wait(kOFree + drain, (outs - 1) & 1);
+            ++outs;
+          }
+          tmem_fence_after();
+        };
+        while (ok && next_work_one()) {
+          const int blocks = max(w.n0, w.n1);
+          if (blocks <= 0) continue;
+          ok = wait(kQFull, loaded & 1);
+          ++loaded;
+          if constexpr (kTiles == 2) {
+            if (ok) {
+              const uint32_t k = take();
+              if (!ok) break;
+              if (w.n0 > 0) {
+                qk(0, sq, k, true);
+                umma_commit(bar(kSFull));
+              }
+              if (w.n1 > 0) {
+                qk(128, sq + kStageBytes, k, true);
+                umma_commit(bar(kSFull + 1));
+              }
+              done();
+              if (blocks == 1) umma_commit(bar(kQFree));
+            }
+            for (int j = 0; j < blocks && ok; ++j) {
+              const uint32_t v = take();
+              if (!ok) break;
+              const int v_slot = slot;
+              step();
+              trim(v_slot, j);
+              const bool more = j + 1 < blocks;
+              uint32_t k = 0;
+              if (j < w.n0) {
+                weights(0, fed0, fed0, 0, out0, j == 0);
+                if (!ok) break;
+                pv(S::kColO, 0, v, j == 0);
+                if (j + 1 == w.n0) umma_commit(bar(kODone));
+              }
+              if (more) k = take();
+              if (!ok) break;
+              if (j + 1 < w.n0) {
+                qk(0, sq, k, true);
+                umma_commit(bar(kSFull));
+              }
+              if (j < w.n1) {
+                weights(1, fed1, fed1, 1, out1, j == 0);
+                if (!ok) break;
+                pv(S::kColO + 128, 128, v, j == 0);
+                if (j + 1 == w.n1) umma_commit(bar(kODone + 1));
+              }
+              umma_commit(bar(kEmpty + v_slot));
+              if (j + 1 < w.n1) {
+                qk(128, sq + kStageBytes, k, true);
+                umma_commit(bar(kSFull + 1));
+              }
+              if (more) {
+                done();
+                if (j + 2 == blocks) umma_commit(bar(kQFree));
+              }
+            }
+          } else {
+            int scored = fed0;
+            auto scores = [&](int j) {
+              for (int h = 0; h < kHalves && ok; ++h) {
+                const uint32_t k = take();
+                if (!ok) return;
+                qk(128 * (scored & 1), sq + h * kStageBytes, k, h == 0);
+                done();
+              }
+              if (!ok) return;
+              umma_commit(bar(kSFull + (scored & 1)));
+              if (j + 1 == blocks) umma_commit(bar(kQFree));
+              ++scored;
+            };
+            if (ok) scores(0);
+            for (int j = 0; j < blocks && ok; ++j) {
+              if (j + 1 < blocks) scores(j + 1);
+              const int buf = fed0 & 1;
+              weights(buf, fed0, fed0 >> 1, 0, out0, j == 0);
+              for (int h = 0; h < kHalves && ok; ++h) {
+                const uint32_t v = take();
+                if (!ok) break;
+                trim(slot, j);
+                if (!ok) break;
+                pv(S::kColO + 128 * h, 128 * buf, v, j == 0);
+                done();
+              }
+              if (ok) umma_commit(bar(kODone));
+            }
+          }
+        }
+        if (abort_flag) {
+          // Given up: let the MMAs in flight end before their memory goes.
+          umma_commit(bar(kDrain));
+          const uint64_t t0 = globaltimer_ns();
+          while (!mbar_try_wait(bar(kDrain), 0) && globaltimer_ns() - t0 < kStallTimeoutNs) {
+          }
+        }
+      }
+      __syncwarp();
+    } else if (warp == S::kTrimWarp) {
+      // -------------------------------------------------------- trimming
+      // V rows behind the sequence's end become zeros before the MMA warp,
+      // which waits for this, multiplies them by zero weights.
+      bool ok = true;
+      int gone = 0;
+      while (ok && next_work()) {
+        const int blocks = max(w.n0, w.n1);
+        if (blocks <= 0 || blocks * kKeys <= w.nk) continue;
+        for (int h = 0; h < kHalves && ok; ++h, ++gone) {
+          ok = wait_warp(kTrimGo, gone & 1);
+          if (!ok) break;
+          const uint32_t v = trim_at.x;
+          const int have = (int)trim_at.y;
+          for (int e = lane; e < (kKeys - have) * 16; e += 32) {
+            const uint32_t at =
+                v + (e & 1) * kBlockBytes + (have + (e >> 4)) * 128 + ((e >> 1) & 7) * 16;
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
+          }
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(kTrimmed));
+        }
+      }
+    }
   }
   __syncthreads();
-  if (warp == S::kSoftWarps + 1) tmem_free(tmem, 512);
+  if (warp == S::kMmaWarp) tmem_free(tmem, 512);
 }
 
 using PromptFn = void (*)(const PromptParams);
