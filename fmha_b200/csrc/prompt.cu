@@ -67,7 +67,6 @@ struct PromptParams {
   float scale_log2;
   int causal;
   int pack_log2;  // PACK
-  int o_bf16;
   unsigned int* err;
 };
 
@@ -86,8 +85,9 @@ struct PromptShape {
                        kTrimWarp = kPlanWarp + 1;
   static constexpr int kThreads = 32 * (kSoftWarps + 4);
   static constexpr int kQBytes = 2 * kStageBytes;    // either two tiles or two halves
-  static constexpr int kStages = 5;
-  static constexpr int kSmem = kQBytes + kStages * kStageBytes + 1024;  // aligned to 1024 inside
+  static constexpr int kStages = 4;
+  static constexpr int kOutBytes = kSoftWarps * 4096;  // 32 rows x 64 columns of output per warp
+  static constexpr int kSmem = kQBytes + kStages * kStageBytes + kOutBytes + 1024;  // aligned inside
   static constexpr uint32_t kColO = 256;             // S buffers at 0 and 128
 };
 
@@ -160,7 +160,7 @@ __device__ __forceinline__ int tile_blocks(const PromptParams& P, const Work& w,
 // One output row on the CUDA cores, by one warp: weights 2^(s*sc + neg) over
 // the row's own `seen` keys, divided by l. For rows that met a NaN or an
 // infinity behind their last key in the tensor cores.
-template <int D, bool BF16>
+template <int D, bool BF16, bool OUT_BF16>
 __device__ __noinline__ void row_again(const PromptParams& P, int64_t q_row, int64_t k_row, int head,
                                        int kvh, int seen, float neg, float l) {
   constexpr int kMine = D / 32;  // columns of a lane
@@ -197,15 +197,78 @@ __device__ __noinline__ void row_again(const PromptParams& P, int64_t q_row, int
 #pragma unroll
   for (int i = 0; i < kMine / 2; ++i) {
     const float a = o[2 * i] / l, b = o[2 * i + 1] / l;
-    out[i] = P.o_bf16 ? pack2<true>(a, b) : pack2<false>(a, b);
+    out[i] = pack2<OUT_BF16>(a, b);
   }
 }
 
-template <int D, bool BF16, bool SPLIT>
+// A tile's output from tensor memory (o_at; 0: nothing there, all zeros) to
+// global memory, one thread to a row's arithmetic; arrives on `drained` once
+// it is read. Returns whether the thread's row has a NaN. 64 columns at a time
+// go through shared memory (4 KB per warp), so that the warp writes rows of
+// 128 adjacent bytes.
+template <int D, bool OUT_BF16>
+__device__ __forceinline__ bool write_tile(const PromptParams& P, uint32_t o_at, uint32_t out_at,
+                                           uint32_t drained, int64_t q_row, int tokens_left,
+                                           int head0, bool none, float inv) {
+  const int lane = threadIdx.x & 31, row0 = threadIdx.x & 96;
+  const int pack_mask = (1 << P.pack_log2) - 1;
+  // Rows row0 + r, r = 4i + lane/8, of the lane's stores.
+  uint16_t* const out = P.o + q_row * P.o_stride + (int64_t)head0 * D + 8 * (lane & 7);
+  const int stride = (int)P.o_stride;  // below 2^31
+  const float2 inv2 = make_float2(inv, inv);
+  float2 bad = make_float2(0.0f, 0.0f);  // stays 0 unless something is NaN (or infinite: 0 * inf)
+#pragma unroll 1
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t y[32];
+    if (o_at) {
+      tmem_ld32(y, o_at + 32 * c);
+      tmem_wait_ld(y);
+      if (c + 1 == D / 32) {  // the next output may take its place
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(drained);
+      }
+    }
+    if (none || !o_at) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) y[i] = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t z[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 a = mul2(make_float2(__uint_as_float(y[8 * i + 2 * e]),
+                                          __uint_as_float(y[8 * i + 2 * e + 1])), inv2);
+        bad = fma2(a, make_float2(0.0f, 0.0f), bad);
+        z[e] = pack2<OUT_BF16>(a.x, a.y);
+      }
+      asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
+                       out_at + lane * 128 + (((4 * (c & 1) + i) ^ (lane & 7)) << 4)),
+                   "r"(z[0]), "r"(z[1]), "r"(z[2]), "r"(z[3])
+                   : "memory");
+    }
+    __syncwarp();
+    if ((c & 1) == 0) continue;
+#pragma unroll 4
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + (lane >> 3);  // of the warp
+      const int t = (row0 + r) >> P.pack_log2, h = (row0 + r) & pack_mask;
+      const uint4 z = lds128(out_at + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+      if (t < tokens_left)
+        *reinterpret_cast<uint4*>(out + (int64_t)t * stride + h * D + 32 * (c - 1)) = z;
+    }
+    __syncwarp();
+  }
+  return isnan(bad.x) || isnan(bad.y);
+}
+
+template <int D, bool BF16, bool OUT_BF16>
 __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
     prompt_kernel(const __grid_constant__ PromptParams P) {
   using S = PromptShape<D>;
   constexpr int kTiles = S::kTiles, kHalves = S::kHalves, kStages = S::kStages;
+  constexpr bool SPLIT = BF16 && !OUT_BF16;
   // Weights in fp16 carry 2^7, so that small ones keep clear of its short exponent.
   constexpr float kShift = BF16 ? 0.0f : 7.0f;
   // Barriers: ring stages filled and free; Q in and free; scores ready and
@@ -217,7 +280,8 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
     kQFull = kEmpty + S::kStages,
     kQFree,
     kSFull,
-    kPFull = kSFull + 2,
+    kPMost = kSFull + 2,  // of all keys but 32..63
+    kPFull = kPMost + 2,
     kODone = kPFull + 2,
     kOFree = kODone + 2,
     kWorkFull = kOFree + 2,
@@ -246,7 +310,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
       abort_flag = 0;
       for (int i = 0; i < kBars; ++i) {
         int count = 1;
-        if ((i >= kPFull && i < kPFull + 2) || (i >= kOFree && i < kOFree + 2)) count = 4;
+        if ((i >= kPMost && i < kPFull + 2) || (i >= kOFree && i < kOFree + 2)) count = 4;
         if (i >= kWorkFree && i < kWorkFree + 2) count = S::kSoftWarps + 3;  // TMA, MMA, trim
         mbar_init(bar(i), count);
       }
@@ -313,46 +377,64 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
       const int warp_tok = tok_base + ((row & ~31) >> P.pack_log2);
       const int least = P.causal ? min(w.nk, warp_tok + ahead + 1) : w.nk;  // of the warp's first row
       float m = -INFINITY, l = 0.0f;
+#pragma unroll 1
       for (int j = 0; j < n; ++j, ++block) {
         const int buf = kTiles == 2 ? tile : block & 1;
         ok = wait_warp(kSFull + buf, kTiles == 2 ? block & 1 : (block >> 1) & 1);
         if (!ok) break;
         tmem_fence_after();
         const uint32_t s_at = lanes + 128 * buf;
-        uint32_t x[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(x[c], s_at + 32 * c);
-        tmem_wait_ld();
-        if ((j + 1) * kKeys > least) {
-          const int left = seen - j * kKeys;
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
+        // 32 scores at a time. The maximum is taken over keys 0..63, then
+        // 64..127, which stay in registers; 0..63 are read again for their
+        // weights. Weights go where their scores were: those of 32 keys take
+        // the first 16 of their 32 columns (low parts the other 16).
+        uint32_t xa[32], xb[32], xc[32];
+        const bool cut = (j + 1) * kKeys > least;  // some row of the warp ends in this block
+        const int left = seen - j * kKeys;
+        auto mask = [&](uint32_t (&x)[32], int first) {
+          if (cut) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (32 * c + i >= left) x[c][i] = 0xff800000u;
-        }
+              if (first + i >= left) x[i] = 0xff800000u;
+          }
+        };
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto highest = [&](const uint32_t (&x)[32]) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], __uint_as_float(x[c][i]));
-        const float now = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
-        if (j == 0) {
-          m = now;
-        } else {
-          const bool rise = (now - m) * sc > kSlack;
-          if (__any_sync(kFullMask, rise)) {
+          for (int i = 0; i < 32; i += 2)
+            top[(i >> 1) & 3] = max3(top[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+        };
+        tmem_ld32(xa, s_at);
+        tmem_ld32(xb, s_at + 32);
+        tmem_wait_ld(xa);
+        tmem_wait_ld(xb);
+        mask(xa, 0);
+        mask(xb, 32);
+        highest(xa);
+        highest(xb);
+        tmem_ld32(xa, s_at + 64);
+        tmem_ld32(xb, s_at + 96);
+        tmem_wait_ld(xa);
+        tmem_wait_ld(xb);
+        mask(xa, 64);
+        mask(xb, 96);
+        highest(xa);
+        highest(xb);
+        const float now = max3(m, max3(top[0], top[1], top[2]), top[3]);
+        const bool rise = (now - m) * sc > kSlack;  // in the first block of all rows with a key
+        if (__any_sync(kFullMask, rise)) {
+          float f = 1.0f;
+          if (rise) {
+            f = ex2((m - now) * sc);
+            m = now;
+            l *= f;
+          }
+          if (j > 0) {
             // The scores of block j follow P.V of block j-1 (head_dim 128), or of j-2 (256).
             if (kTiles == 1) {
               ok = wait_warp(kODone, (block - 1) & 1);
               if (!ok) break;
               tmem_fence_after();
-            }
-            float f = 1.0f;
-            if (rise) {
-              f = ex2((m - now) * sc);
-              m = now;
-              l *= f;
             }
             __syncwarp();
 #pragma unroll 1
@@ -367,32 +449,40 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
           }
         }
         const float neg = m == -INFINITY ? 0.0f : kShift - m * sc;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const float2 sc2 = make_float2(sc, sc), neg2 = make_float2(neg, neg);
+        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        auto weigh = [&](const uint32_t (&x)[32], int first) {
+          uint32_t hi[16], lo[SPLIT ? 16 : 1];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float p = ex2(fmaf(__uint_as_float(x[c][i]), sc, neg));
-            sum[i & 3] += p;
-            x[c][i] = __float_as_uint(p);
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t hi[32], lo[SPLIT ? 32 : 1];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float a = __uint_as_float(x[2 * c + (i >> 4)][(2 * i) & 31]);
-            const float b = __uint_as_float(x[2 * c + (i >> 4)][((2 * i) & 31) + 1]);
+          for (int i = 0; i < 16; ++i) {
+            float2 p = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), sc2, neg2);
+            p = make_float2(ex2(p.x), ex2(p.y));
+            sum[i & 1] = add2(sum[i & 1], p);
             if constexpr (SPLIT)
-              split2<BF16>(a, b, hi[i], lo[i]);
+              split2<BF16>(p.x, p.y, hi[i], lo[i]);
             else
-              hi[i] = pack2<BF16>(a, b);
+              hi[i] = pack2<BF16>(p.x, p.y);
           }
-          tmem_st32(s_at + 32 * c, hi);
-          if constexpr (SPLIT) tmem_st32(s_at + 64 + 32 * c, lo);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_st16(s_at + first, hi);
+          if constexpr (SPLIT) tmem_st16(s_at + first + 16, lo);
+        };
+        tmem_ld32(xc, s_at);
+        weigh(xa, 64);
+        weigh(xb, 96);
+        tmem_wait_ld(xc);
+        tmem_ld32(xa, s_at + 32);
+        mask(xc, 0);
+        weigh(xc, 0);
+        // P.V of all keys but 32..63 may start.
+        tmem_wait_st();
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kPMost + buf));
+        tmem_wait_ld(xa);
+        mask(xa, 32);
+        weigh(xa, 32);
+        sum[0] = add2(sum[0], sum[1]);
+        l += sum[0].x + sum[0].y;
         tmem_wait_st();
         tmem_fence_before();
         __syncwarp();
@@ -414,47 +504,20 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
       const bool mine = tok < w.nq;
       const int head = w.head0 + (row & ((1 << P.pack_log2) - 1));
       const bool none = seen == 0;
-      const float inv = 1.0f / l;
-      uint16_t* const out = P.o + (int64_t)(w.q0 + tok) * P.o_stride + (int64_t)head * D;
-      bool nan = false;
-#pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t y[32];
-        if (n > 0) {
-          tmem_ld32(y, o_at + 32 * c);
-          tmem_wait_ld();
-          if (c + 1 == D / 32) {  // the next output may take its place
-            tmem_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(kOFree + (kTiles == 2 ? tile : 0)));
-          }
-        }
-        if (mine) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t z[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float a = none ? 0.0f : __uint_as_float(y[8 * i + 2 * e]) * inv;
-              const float b = none ? 0.0f : __uint_as_float(y[8 * i + 2 * e + 1]) * inv;
-              nan |= isnan(a) || isnan(b);
-              z[e] = P.o_bf16 ? pack2<true>(a, b) : pack2<false>(a, b);
-            }
-            *reinterpret_cast<uint4*>(out + 32 * c + 8 * i) = make_uint4(z[0], z[1], z[2], z[3]);
-          }
-        }
-        __syncwarp();
-      }
+      const bool nan = write_tile<D, OUT_BF16>(
+          P, n > 0 ? o_at : 0u, ring + kStages * kStageBytes + warp * 4096,
+          bar(kOFree + (kTiles == 2 ? tile : 0)), w.q0 + tok_base, w.nq - tok_base, w.head0, none,
+          none ? 0.0f : 1.0f / l);
       if (mine && P.lse)
         P.lse[(int64_t)(w.q0 + tok) * P.hq + head] =
             none ? -INFINITY : (m * sc + (log2f(l) - kShift)) * 0.69314718055994531f;
       // NaN in rows whose weights are sound (l = 0: every score -inf, 0/0).
-      unsigned again = __ballot_sync(kFullMask, nan && l > 0.0f && l <= FLT_MAX);
+      unsigned again = __ballot_sync(kFullMask, mine && nan && l > 0.0f && l <= FLT_MAX);
       const float neg = m == -INFINITY ? 0.0f : kShift - m * sc;
       while (again) {
         const int r = __ffs(again) - 1;
         again &= again - 1;
-        row_again<D, BF16>(P, w.q0 + __shfl_sync(kFullMask, tok, r), w.k0,
+        row_again<D, BF16, OUT_BF16>(P, w.q0 + __shfl_sync(kFullMask, tok, r), w.k0,
                            __shfl_sync(kFullMask, head, r), w.kvh, __shfl_sync(kFullMask, seen, r),
                            __shfl_sync(kFullMask, neg, r), __shfl_sync(kFullMask, l, r));
       }
@@ -597,15 +660,18 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
             umma_ss(tmem + s_col, a + off, b + off, kIdQK, !(first && i == 0));
           }
         };
-        // O += P V over one 128-column part.
-        auto pv = [&](uint32_t o_col, uint32_t p_col, uint32_t v, bool first) {
+        // O += P V over one 128-column part: keys 64..127 and 0..31, or 32..63.
+        auto pv = [&](uint32_t o_col, uint32_t p_col, uint32_t v, bool most, bool first) {
           const uint64_t b = umma_desc(v, kBlockBytes, 1024);
 #pragma unroll
           for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              umma_ts(tmem + o_col, tmem + p_col + part * 64 + i * 8, b + ((i * 2048) >> 4), kIdPV,
-                      !(first && part == 0 && i == 0));
+            for (int n = 0; n < 8; ++n) {
+              const int i = (n + 4) & 7;  // 16 keys
+              if ((i >> 1 == 1) == most) continue;
+              umma_ts(tmem + o_col, tmem + p_col + 32 * (i >> 1) + 16 * part + 8 * (i & 1),
+                      b + ((i * 2048) >> 4), kIdPV, !(first && part == 0 && n == 0));
+            }
         };
         // V rows behind the sequence's end, if block j has any, are cleared by
         // the trimming warp.
@@ -617,15 +683,18 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
           ok = wait(kTrimmed, trimmed & 1);
           ++trimmed;
         };
-        // Waits for the next weights of tile (or buffer) i, and before the
-        // first of a piece for the last output of that tile to be drained.
-        auto weights = [&](int b, int& fed, int parity, int drain, int& outs, bool first) {
-          ok = ok && wait(kPFull + b, parity & 1);
-          ++fed;
+        // Waits for the next weights in buffer b, most of them; and before
+        // the first of a piece for the last output of that tile to be drained.
+        auto weights = [&](int b, int parity, int drain, int& outs, bool first) {
+          ok = ok && wait(kPMost + b, parity & 1);
           if (first) {
             if (outs > 0) ok = ok && wait(kOFree + drain, (outs - 1) & 1);
             ++outs;
           }
+          tmem_fence_after();
+        };
+        auto other_weights = [&](int b, int parity) {
+          ok = ok && wait(kPFull + b, parity & 1);
           tmem_fence_after();
         };
         while (ok && next_work_one()) {
@@ -657,9 +726,12 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
               const bool more = j + 1 < blocks;
               uint32_t k = 0;
               if (j < w.n0) {
-                weights(0, fed0, fed0, 0, out0, j == 0);
+                weights(0, fed0, 0, out0, j == 0);
                 if (!ok) break;
-                pv(S::kColO, 0, v, j == 0);
+                pv(S::kColO, 0, v, true, j == 0);
+                other_weights(0, fed0++);
+                if (!ok) break;
+                pv(S::kColO, 0, v, false, false);
                 if (j + 1 == w.n0) umma_commit(bar(kODone));
               }
               if (more) k = take();
@@ -669,9 +741,12 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
                 umma_commit(bar(kSFull));
               }
               if (j < w.n1) {
-                weights(1, fed1, fed1, 1, out1, j == 0);
+                weights(1, fed1, 1, out1, j == 0);
                 if (!ok) break;
-                pv(S::kColO + 128, 128, v, j == 0);
+                pv(S::kColO + 128, 128, v, true, j == 0);
+                other_weights(1, fed1++);
+                if (!ok) break;
+                pv(S::kColO + 128, 128, v, false, false);
                 if (j + 1 == w.n1) umma_commit(bar(kODone + 1));
               }
               umma_commit(bar(kEmpty + v_slot));
@@ -702,13 +777,16 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
             for (int j = 0; j < blocks && ok; ++j) {
               if (j + 1 < blocks) scores(j + 1);
               const int buf = fed0 & 1;
-              weights(buf, fed0, fed0 >> 1, 0, out0, j == 0);
+              weights(buf, fed0 >> 1, 0, out0, j == 0);
               for (int h = 0; h < kHalves && ok; ++h) {
                 const uint32_t v = take();
                 if (!ok) break;
                 trim(slot, j);
                 if (!ok) break;
-                pv(S::kColO + 128 * h, 128 * buf, v, j == 0);
+                pv(S::kColO + 128 * h, 128 * buf, v, true, j == 0);
+                if (h == 0) other_weights(buf, fed0++ >> 1);
+                if (!ok) break;
+                pv(S::kColO + 128 * h, 128 * buf, v, false, false);
                 done();
               }
               if (ok) umma_commit(bar(kODone));
@@ -757,9 +835,9 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
 using PromptFn = void (*)(const PromptParams);
 
 template <int D>
-PromptFn prompt_fn(bool bf16, bool split) {
-  if (!bf16) return prompt_kernel<D, false, false>;
-  return split ? prompt_kernel<D, true, true> : prompt_kernel<D, true, false>;
+PromptFn prompt_fn(bool bf16, bool out_bf16) {
+  if (bf16) return out_bf16 ? prompt_kernel<D, true, true> : prompt_kernel<D, true, false>;
+  return out_bf16 ? prompt_kernel<D, false, true> : prompt_kernel<D, false, false>;
 }
 
 // The driver's tensor-map encoder, looked up once.
@@ -821,6 +899,7 @@ extern "C" fmha_status_t fmha_prompt(const fmha_prompt_args_t* args, fmha_stream
   if (keys && ((st = check_rows(A.k, A.k_stride, hkv, d)) != FMHA_OK ||
                (st = check_rows(A.v, A.v_stride, hkv, d)) != FMHA_OK))
     return st;
+  if (A.o_stride > 0x7fffffff) return FMHA_ERR_UNSUPPORTED;
   if (!A.cu_seqlens_q) return FMHA_ERR_INVALID_ARG;
   if (!A.cu_seqlens_kv && A.total_kv != A.total_q) return FMHA_ERR_INVALID_ARG;
   if ((reinterpret_cast<uintptr_t>(A.lse) | reinterpret_cast<uintptr_t>(A.cu_seqlens_q) |
@@ -850,7 +929,6 @@ extern "C" fmha_status_t fmha_prompt(const fmha_prompt_args_t* args, fmha_stream
       A.softmax_scale > 0.0f ? (double)A.softmax_scale : 1.0 / std::sqrt((double)d);
   P.scale_log2 = (float)(1.4426950408889634 * scale);
   P.causal = A.causal != 0;
-  P.o_bf16 = A.o_dtype == FMHA_DTYPE_BF16;
   P.err = dev.err;
   const bool bf16 = A.dtype == FMHA_DTYPE_BF16;
   const int g = hq / hkv;
@@ -863,8 +941,8 @@ extern "C" fmha_status_t fmha_prompt(const fmha_prompt_args_t* args, fmha_stream
       !encode(&P.map_v, bf16, keys ? A.v : A.q, d, keys ? hkv : hq,
               keys ? A.total_kv : A.total_q, keys ? A.v_stride : A.q_stride, 1, kKeys))
     return FMHA_ERR_CUDA;
-  const bool split = bf16 && !P.o_bf16;
-  const PromptFn fn = d == 128 ? prompt_fn<128>(bf16, split) : prompt_fn<256>(bf16, split);
+  const bool out_bf16 = A.o_dtype == FMHA_DTYPE_BF16;
+  const PromptFn fn = d == 128 ? prompt_fn<128>(bf16, out_bf16) : prompt_fn<256>(bf16, out_bf16);
   const int smem = d == 128 ? PromptShape<128>::kSmem : PromptShape<256>::kSmem;
   const int threads = d == 128 ? PromptShape<128>::kThreads : PromptShape<256>::kThreads;
   if ((st = ensure_smem(reinterpret_cast<const void*>(fn), smem)) != FMHA_OK) return st;

@@ -100,7 +100,7 @@ def test_decode_refuses(kw, status):
     (dict(o=72), MISALIGNED), (dict(o_stride=4092), INVALID), (dict(lse=2), MISALIGNED),
     (dict(cu_seqlens_q=0), INVALID), (dict(cu_seqlens_q=130), MISALIGNED), (dict(cu_seqlens_kv=131), MISALIGNED),
     (dict(total_kv=10), INVALID), (dict(o_dtype=E4M3), UNSUPPORTED), (dict(softmax_scale=-0.5), INVALID),
-    (dict(softmax_scale=NAN), INVALID),
+    (dict(softmax_scale=NAN), INVALID), (dict(o_stride=1 << 31), UNSUPPORTED),
 ])
 def test_prompt_refuses(kw, status):
     assert prompt(**kw) == status
