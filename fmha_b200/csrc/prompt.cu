@@ -100,52 +100,123 @@ struct Work {
   int last;            // nothing, and nothing follows
 };
 
-// Piece `index` of the work: tiles of one sequence go from its end to its
-// start, the longest first. False behind the last tile. One warp.
-__device__ bool find_work(const PromptParams& P, int index, int tokens, Work* out) {
-  const int lane = threadIdx.x & 31;
-  const int groups = P.hq >> P.pack_log2;
-  const int group = index % groups;
-  int at = index / groups;
-  for (int b0 = 0; b0 < P.batch; b0 += 32) {
-    const int b = b0 + lane;
-    int64_t len = 0;
-    if (b < P.batch) len = (int64_t)P.cu_q[b + 1] - P.cu_q[b];
+// The list of all pieces (`tokens` tokens of a sequence, of one head group).
+// Up to kSorted sequences it goes by the tokens' place, the last places
+// first: with a causal mask the longest pieces come first and the card ends
+// evenly (29 ragged prompts: 138 us in the
+// sequences' order, 113 us so). The
+// planning warp keeps the sequences' piece counts, 8 to a lane. More
+// sequences go one after the other, each from its end to its start.
+constexpr int kSorted = 256;
+
+struct WorkList {
+  int parts[kSorted / 32];  // of sequences lane, lane + 32, ..
+  int all, places;          // pieces, and the most of a sequence
+
+  // Pieces of sequence b; one impossible at the head of the list is reported.
+  __device__ static int parts_of(const PromptParams& P, int b, int tokens) {
+    if (b >= P.batch) return 0;
+    const int64_t len = (int64_t)P.cu_q[b + 1] - P.cu_q[b];
     if (len < 0 || len > P.total_q) {
       report_device_error(P.err, FMHA_ERR_INVALID_ARG, kSitePromptLength);
-      len = 0;
+      return 0;
     }
-    const int n = (int)((len + tokens - 1) / tokens);
-    int inc = n;
+    return (int)((len + tokens - 1) / tokens);
+  }
+  __device__ void load(const PromptParams& P, int tokens) {
 #pragma unroll
-    for (int s = 1; s < 32; s <<= 1) {
-      const int y = __shfl_up_sync(kFullMask, inc, s);
-      if (lane >= s) inc += y;
-    }
-    const unsigned hit = __ballot_sync(kFullMask, at < inc);
-    if (hit) {
-      const int w = __ffs(hit) - 1;
-      const int tile = __shfl_sync(kFullMask, inc, w) - 1 - at;  // reversed inside the sequence
-      const int seq = b0 + w;
-      const int64_t q0 = P.cu_q[seq], nq = P.cu_q[seq + 1] - q0;
-      const int64_t k0 = P.cu_kv[seq], nk = P.cu_kv[seq + 1] - k0;
-      if (q0 < 0 || q0 + nq > P.total_q || k0 < 0 || nk < 0 || k0 + nk > P.total_kv) {
-        if (lane == 0) report_device_error(P.err, FMHA_ERR_INVALID_ARG, kSitePromptLength);
-        return false;
+    for (int k = 0; k < kSorted / 32; ++k)
+      parts[k] = 32 * k < P.batch ? parts_of(P, 32 * k + (threadIdx.x & 31), tokens) : 0;
+    all = from_place(0);
+    places = 0;
+#pragma unroll
+    for (int k = 0; k < kSorted / 32; ++k) places = max(places, parts[k]);
+    places = __reduce_max_sync(kFullMask, places);
+  }
+  // Pieces at place t or later.
+  __device__ int from_place(int t) const {
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < kSorted / 32; ++k) n += max(0, parts[k] - t);
+    return __reduce_add_sync(kFullMask, n);
+  }
+  // Sequence and place of piece `at`; false behind the last. One warp.
+  __device__ bool sorted(int at, int* seq, int* place) const {
+    if (at >= all) return false;
+    if (places == all) {  // one sequence
+      *place = all - 1 - at;
+      *seq = 0;
+#pragma unroll
+      for (int k = 0; k < kSorted / 32; ++k) {
+        const unsigned has = __ballot_sync(kFullMask, parts[k] > 0);
+        if (has) *seq = 32 * k + __ffs(has) - 1;
       }
-      out->q0 = (int)q0;
-      out->nq = (int)nq;
-      out->k0 = (int)k0;
-      out->nk = (int)nk;
-      out->tok0 = tile * tokens;
-      out->head0 = group << P.pack_log2;
-      out->kvh = out->head0 / (P.hq / P.hkv);
       return true;
     }
-    at -= __shfl_sync(kFullMask, inc, 31);
+    int lo = 0, hi = places;  // from_place(lo) > at >= from_place(hi)
+    while (hi - lo > 1) {
+      const int m = (lo + hi) >> 1;
+      if (from_place(m) > at) lo = m; else hi = m;
+    }
+    at -= from_place(hi);  // the at-th sequence that has place lo
+#pragma unroll
+    for (int k = 0; k < kSorted / 32; ++k) {
+      const unsigned has = __ballot_sync(kFullMask, parts[k] > lo);
+      const int n = __popc(has);
+      if (at < n) {
+        const int lane = threadIdx.x & 31;
+        const bool mine = (has >> lane & 1u) && __popc(has & ((1u << lane) - 1)) == at;
+        *seq = 32 * k + __ffs(__ballot_sync(kFullMask, mine)) - 1;
+        *place = lo;
+        return true;
+      }
+      at -= n;
+    }
+    return false;
   }
-  return false;
-}
+  __device__ static bool in_order(const PromptParams& P, int at, int tokens, int* seq, int* place) {
+    const int lane = threadIdx.x & 31;
+    for (int b0 = 0; b0 < P.batch; b0 += 32) {
+      const int n = parts_of(P, b0 + lane, tokens);
+      int inc = n;
+#pragma unroll
+      for (int s = 1; s < 32; s <<= 1) {
+        const int y = __shfl_up_sync(kFullMask, inc, s);
+        if (lane >= s) inc += y;
+      }
+      const unsigned hit = __ballot_sync(kFullMask, at < inc);
+      if (hit) {
+        const int w = __ffs(hit) - 1;
+        *seq = b0 + w;
+        *place = __shfl_sync(kFullMask, inc, w) - 1 - at;
+        return true;
+      }
+      at -= __shfl_sync(kFullMask, inc, 31);
+    }
+    return false;
+  }
+  __device__ bool find(const PromptParams& P, int index, int tokens, Work* out) const {
+    const int groups = P.hq >> P.pack_log2;
+    const int at = index / groups, group = index - at * groups;
+    int seq, place;
+    if (!(P.batch <= kSorted ? sorted(at, &seq, &place) : in_order(P, at, tokens, &seq, &place)))
+      return false;
+    const int64_t q0 = P.cu_q[seq], nq = P.cu_q[seq + 1] - q0;
+    const int64_t k0 = P.cu_kv[seq], nk = P.cu_kv[seq + 1] - k0;
+    if (q0 < 0 || q0 + nq > P.total_q || k0 < 0 || nk < 0 || k0 + nk > P.total_kv) {
+      if ((threadIdx.x & 31) == 0) report_device_error(P.err, FMHA_ERR_INVALID_ARG, kSitePromptLength);
+      return false;
+    }
+    out->q0 = (int)q0;
+    out->nq = (int)nq;
+    out->k0 = (int)k0;
+    out->nk = (int)nk;
+    out->tok0 = place * tokens;
+    out->head0 = group << P.pack_log2;
+    out->kvh = out->head0 / (P.hq / P.hkv);
+    return true;
+  }
+};
 
 // Key blocks that tile i of the CTA needs; -1 if it holds no row.
 __device__ __forceinline__ int tile_blocks(const PromptParams& P, const Work& w, int i) {
@@ -303,6 +374,11 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
   allow_dependent_launch();
   grid_dependency_wait();
 
+  if (warp == S::kTmaWarp && lane == 0) {
+    prefetch_map(&P.map_q);
+    prefetch_map(&P.map_k);
+    prefetch_map(&P.map_v);
+  }
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](int i) { return bar0 + 8 * i; };
   if (warp == S::kMmaWarp) {
@@ -531,6 +607,8 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
       // started, until there are none.
       int index = blockIdx.x, asked = 0;
       bool ok = true;
+      WorkList list;
+      list.load(P, kTiles * tokens);
       while (ok) {
         if (lane == 0 && index >= 0) {
           fence_async_shared();  // the last answer has been read
@@ -538,7 +616,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
           clc_try_cancel(smem_u32(&answer), bar(kAnswer));
         }
         Work mine;
-        const bool found = index >= 0 && find_work(P, index, kTiles * tokens, &mine);
+        const bool found = index >= 0 && list.find(P, index, kTiles * tokens, &mine);
         if (found || index < 0) {
           mine.last = index < 0;
           if (found) {
