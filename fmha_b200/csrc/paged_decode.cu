@@ -21,7 +21,7 @@
 // by a power of two that puts its largest element just below 2^15.
 //
 // Split. A unit is one (sequence, kv head, up to 16 of its query heads); a
-// tile is 16 of its tokens (32 of an e4m3 cache). All tiles of all units, one
+// tile is 16 of its tokens (32 of an e4m3 cache at head_dim 128). All tiles of all units, one
 // after the other, are dealt out in equal contiguous ranges to the CTAs and
 // within them to the warps, whatever the lengths, so ragged batches and a
 // single long sequence fill the card alike. A unit counts one tile more than
@@ -91,14 +91,20 @@ struct DecodeShape {
   static constexpr int kElem = F8 ? 1 : 2;
   static constexpr int kRowBytes = D * kElem;
   static constexpr int kChunks = kRowBytes / 16;  // 16-byte pieces of a row
-  static constexpr int kSub = F8 && !(WIDE && D == 256) ? 2 : 1;  // 16-token steps of a tile
+  // 16-token steps of a tile, warps, and tiles of a warp's ring. e4m3 tiles
+  // cost twice the instructions per byte, so the warps' latency shows first:
+  // at head_dim 128 two steps at a time overlap (5.3 TB/s, 128 sequences of
+  // 2048 tokens, 32/8 heads; one step 4.3, 12 warps 4.8), at 256 eight warps
+  // (5.5 TB/s, 64 of 4096, 32/16 heads; 4 warps with two steps 4.4, 7 with a
+  // longer ring 4.8).
+  static constexpr int kSub = F8 && D == 128 ? 2 : 1;
   static constexpr int kTile = 16 * kSub;
   static constexpr int kRows = WIDE ? 16 : 8;
   static constexpr int kHalf = kTile * kRowBytes;  // K or V of a tile
   static constexpr int kStage = 2 * kHalf;
-  static constexpr int kWarps = D == 128 ? (WIDE ? 6 : 8) : (F8 && WIDE ? 5 : 4);
+  static constexpr int kWarps = D == 128 ? (WIDE ? 6 : 8) : F8 ? (WIDE ? 5 : 8) : 4;
   static constexpr int kThreads = 32 * kWarps;
-  static constexpr int kStages = D == 256 && WIDE && !F8 ? 2 : 3;
+  static constexpr int kStages = D == 256 && WIDE != F8 ? 2 : 3;
   static constexpr int kPad = D + 4;  // floats of a row of partial results
   static constexpr int kRing = kStages * kStage;  // of a warp
   static constexpr int kHold = kRows * kPad * 4;  // a warp's partial result of its first unit

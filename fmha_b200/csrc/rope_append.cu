@@ -8,14 +8,14 @@
 // written once, so HBM bandwidth bounds long prompts and launch latency a
 // decode step.
 //
-// Split. One thread turns 16 elements of one head: two 16-byte vectors that
-// hold both halves of 8 pairs (for interleaved pairs, and for elements behind
-// rotary_dim, two adjacent vectors). Its chunk of the head is the same for
-// all its heads, so it loads the 8 cosines and sines of a token once for all
-// of them. A block takes a contiguous range of tokens and walks the heads
-// (queries, keys, values) of one token at a time, up to kBatch of them with
-// their loads in flight before the first is used; the token's sequence,
-// position and page are looked up behind those loads.
+// Split. A thread has one token and 16 elements of a head: two 16-byte
+// vectors that hold both halves of 8 pairs (for interleaved pairs, and for
+// elements behind rotary_dim, two adjacent vectors). It walks a range of the
+// token's heads (queries, then keys, then values) with kBatch heads' loads in
+// flight, so the token's sequence, position, page and 8 cosines and sines are
+// looked up once, all tokens' at the same time. Many tokens take a thread
+// row per token (8 or 16 threads); few tokens have their heads dealt to more
+// threads, until kSpread fill the card.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -31,7 +31,8 @@ namespace fmha {
 namespace {
 
 constexpr int kAppendThreads = 256;
-constexpr int kBatch = 2;  // heads in flight per thread
+constexpr int kBatch = 4;             // heads in flight per thread
+constexpr int kSpread = 148 * 1024;   // threads worth dealing the heads to
 
 struct AppendParams {
   const uint16_t* q;
@@ -50,6 +51,8 @@ struct AppendParams {
   int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
   int rot;
   int max_position;
+  int split;  // threads among which a token's heads are dealt
+  float k_inv, v_inv;  // 1 / scale of e4m3 pages
   unsigned int* err;
 };
 
@@ -84,15 +87,16 @@ __device__ __forceinline__ uint4 pack16(const float (&f)[8]) {
   return make_uint4(u[0], u[1], u[2], u[3]);
 }
 
-// 8 values divided by the cache's scale, as saturated e4m3 codes.
-__device__ __forceinline__ uint2 pack_e4m3(const float (&f)[8], float scale) {
+// 8 values over the cache's scale, as saturated e4m3 codes. The product with
+// 1/scale is within 2^-23 of the quotient, which the code keeps 4 bits of.
+__device__ __forceinline__ uint2 pack_e4m3(const float (&f)[8], float inv) {
   uint32_t u[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * i] / scale, f[4 * i + 1] / scale),
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * i] * inv, f[4 * i + 1] * inv),
                                                  __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(
-        make_float2(f[4 * i + 2] / scale, f[4 * i + 3] / scale), __NV_SATFINITE, __NV_E4M3);
+        make_float2(f[4 * i + 2] * inv, f[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
     u[i] = lo | (hi << 16);
   }
   return make_uint2(u[0], u[1]);
@@ -105,158 +109,148 @@ __device__ __forceinline__ uint4 ld16(const uint16_t* p) {
 template <bool BF16, bool F8, bool INTER, int D>
 __global__ void __launch_bounds__(kAppendThreads)
     rope_append_kernel(const __grid_constant__ AppendParams P) {
-  constexpr int kChunks = D / 16;                   // threads of one head
-  constexpr int kSlots = kAppendThreads / kChunks;  // heads side by side
+  constexpr int kChunks = D / 16;  // threads of one head
   allow_dependent_launch();
   grid_dependency_wait();
+  const int64_t idx = (int64_t)blockIdx.x * kAppendThreads + threadIdx.x;
   const int c = threadIdx.x % kChunks;
-  const int slot = threadIdx.x / kChunks;
+  const int64_t rest = idx / kChunks;
+  const int t = (int)(rest / P.split), part = (int)(rest - (int64_t)t * P.split);
+  if (t >= P.total_tokens) return;
+
+  // The token's sequence (the last one that starts at or before t) and position.
+  int b, pos;
+  if (P.cu) {
+    int l = 0, r = P.batch;  // cu[l] <= t < cu[r], if t is anyone's
+    while (r - l > 1) {
+      const int m = (l + r) >> 1;
+      if (P.cu[m] <= t) l = m; else r = m;
+    }
+    b = l;
+    const int start = P.cu[b], end = P.cu[b + 1];
+    if (t < start || t >= end) return;  // behind the last sequence
+    pos = P.cache.seqlens_kv[b] - (end - t);
+    if (pos < t - start) pos = -1;  // fewer tokens than new ones
+  } else {
+    b = t;
+    pos = P.cache.seqlens_kv[b] - 1;
+  }
+  const int in_table = pos / P.cache.page_size;
+  if (pos < 0 || in_table >= P.cache.max_pages || (P.rot > 0 && pos >= P.max_position)) {
+    if (c == 0) report_device_error(P.err, FMHA_ERR_INVALID_ARG, kSiteAppendPosition);
+    return;
+  }
+  const int page = P.cache.block_table[b * P.cache.table_stride + in_table];
   const bool turned = c * 16 < P.rot;
+  float cs[8], sn[8];
+  if (turned) {
+    const int64_t at = (int64_t)pos * (P.rot / 2) + 8 * c;
+    const float4* const pc = reinterpret_cast<const float4*>(P.cos_table + at);
+    const float4* const ps = reinterpret_cast<const float4*>(P.sin_table + at);
+    const float4 c0 = __ldg(pc), c1 = __ldg(pc + 1), s0 = __ldg(ps), s1 = __ldg(ps + 1);
+    cs[0] = c0.x; cs[1] = c0.y; cs[2] = c0.z; cs[3] = c0.w;
+    cs[4] = c1.x; cs[5] = c1.y; cs[6] = c1.z; cs[7] = c1.w;
+    sn[0] = s0.x; sn[1] = s0.y; sn[2] = s0.z; sn[3] = s0.w;
+    sn[4] = s1.x; sn[5] = s1.y; sn[6] = s1.z; sn[7] = s1.w;
+  }
+  if (page < 0 || page >= P.cache.num_pages) {
+    if (c == 0) report_device_error(P.err, FMHA_ERR_INVALID_ARG, kSiteAppendPage);
+    return;
+  }
+  const int64_t row = page * P.cache.page_stride +
+                      (int64_t)(pos - in_table * P.cache.page_size) * P.cache.token_stride;
+
   // Offsets of the thread's two vectors in a rotated head; values keep to
   // adjacent vectors.
   const int lo = !INTER && turned ? 8 * c : 16 * c;
   const int hi = !INTER && turned ? 8 * c + P.rot / 2 : 16 * c + 8;
   const int heads = P.hq + 2 * P.hkv;
-  const int first = blockIdx.y * kSlots + slot;
-  const int step = gridDim.y * kSlots;
+  const int first = (int)((int64_t)heads * part / P.split);
+  const int last = (int)((int64_t)heads * (part + 1) / P.split);
 
-  const int t0 = (int)((int64_t)P.total_tokens * blockIdx.x / gridDim.x);
-  const int t1 = (int)((int64_t)P.total_tokens * (blockIdx.x + 1) / gridDim.x);
-  int b = -1;
-  for (int t = t0; t < t1; ++t) {
-    const uint16_t* const q = P.q + t * P.q_stride;
-    const uint16_t* const k = P.k + t * P.k_stride;
-    const uint16_t* const v = P.v + t * P.v_stride;
-    auto source = [&](int h, int off, bool second) {
-      if (h < P.hq) return q + (int64_t)h * D + off;
-      if (h < P.hq + P.hkv) return k + (int64_t)(h - P.hq) * D + off;
-      return v + (int64_t)(h - P.hq - P.hkv) * D + 16 * c + (second ? 8 : 0);
-    };
-    uint4 x[kBatch][2];
+  auto turn = [&](uint4& v0, uint4& v1, float (&a)[8], float (&z)[8]) {
+    unpack16<BF16>(v0, a);
+    unpack16<BF16>(v1, z);
+    if constexpr (INTER) {
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int h = first + i * step;
-      if (h < heads) {
-        x[i][0] = ld16(source(h, lo, false));
-        x[i][1] = ld16(source(h, hi, true));
+      for (int i = 0; i < 4; ++i) {
+        const float a1 = a[2 * i], a2 = a[2 * i + 1], z1 = z[2 * i], z2 = z[2 * i + 1];
+        a[2 * i] = a1 * cs[i] - a2 * sn[i];
+        a[2 * i + 1] = a2 * cs[i] + a1 * sn[i];
+        z[2 * i] = z1 * cs[4 + i] - z2 * sn[4 + i];
+        z[2 * i + 1] = z2 * cs[4 + i] + z1 * sn[4 + i];
       }
-    }
-
-    // The token's sequence (the last one that starts at or before t),
-    // position, page and angles.
-    int pos;
-    if (P.cu) {
-      if (b < 0) {
-        int l = 0, r = P.batch;  // cu[l] <= t < cu[r], if t is anyone's
-        while (r - l > 1) {
-          const int m = (l + r) >> 1;
-          if (P.cu[m] <= t) l = m; else r = m;
-        }
-        b = l;
-      }
-      while (b + 1 < P.batch && P.cu[b + 1] <= t) ++b;
-      const int end = P.cu[b + 1];
-      if (t < P.cu[b] || t >= end) continue;  // behind the last sequence
-      pos = P.cache.seqlens_kv[b] - (end - t);
-      if (pos < t - P.cu[b]) pos = -1;  // fewer tokens than new ones
     } else {
-      b = t;
-      pos = P.cache.seqlens_kv[b] - 1;
-    }
-    const int in_table = pos / P.cache.page_size;
-    if (pos < 0 || in_table >= P.cache.max_pages || (P.rot > 0 && pos >= P.max_position)) {
-      if (threadIdx.x == 0) report_device_error(P.err, FMHA_ERR_INVALID_ARG, kSiteAppendPosition);
-      continue;
-    }
-    const int page = P.cache.block_table[b * P.cache.table_stride + in_table];
-    if (page < 0 || page >= P.cache.num_pages) {
-      if (threadIdx.x == 0) report_device_error(P.err, FMHA_ERR_INVALID_ARG, kSiteAppendPage);
-      continue;
-    }
-    const int64_t row = page * P.cache.page_stride +
-                        (int64_t)(pos - in_table * P.cache.page_size) * P.cache.token_stride;
-    float cs[8], sn[8];
-    if (turned) {
-      const int64_t at = (int64_t)pos * (P.rot / 2) + 8 * c;
-      const float4* const pc = reinterpret_cast<const float4*>(P.cos_table + at);
-      const float4* const ps = reinterpret_cast<const float4*>(P.sin_table + at);
-      const float4 c0 = __ldg(pc), c1 = __ldg(pc + 1), s0 = __ldg(ps), s1 = __ldg(ps + 1);
-      cs[0] = c0.x; cs[1] = c0.y; cs[2] = c0.z; cs[3] = c0.w;
-      cs[4] = c1.x; cs[5] = c1.y; cs[6] = c1.z; cs[7] = c1.w;
-      sn[0] = s0.x; sn[1] = s0.y; sn[2] = s0.z; sn[3] = s0.w;
-      sn[4] = s1.x; sn[5] = s1.y; sn[6] = s1.z; sn[7] = s1.w;
-    }
-
-    auto put = [&](int h, const uint4 (&in)[2]) {
-      const bool value = h >= P.hq + P.hkv;
-      float a[8], z[8];
-      uint4 out0 = in[0], out1 = in[1];
-      if (F8 || (turned && !value)) {
-        unpack16<BF16>(in[0], a);
-        unpack16<BF16>(in[1], z);
-      }
-      if (turned && !value) {
-        if constexpr (INTER) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float a1 = a[2 * i], a2 = a[2 * i + 1], z1 = z[2 * i], z2 = z[2 * i + 1];
-            a[2 * i] = a1 * cs[i] - a2 * sn[i];
-            a[2 * i + 1] = a2 * cs[i] + a1 * sn[i];
-            z[2 * i] = z1 * cs[4 + i] - z2 * sn[4 + i];
-            z[2 * i + 1] = z2 * cs[4 + i] + z1 * sn[4 + i];
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float x1 = a[i], x2 = z[i];
-            a[i] = x1 * cs[i] - x2 * sn[i];
-            z[i] = x2 * cs[i] + x1 * sn[i];
-          }
-        }
-        out0 = pack16<BF16>(a);
-        out1 = pack16<BF16>(z);
+      for (int i = 0; i < 8; ++i) {
+        const float x1 = a[i], x2 = z[i];
+        a[i] = x1 * cs[i] - x2 * sn[i];
+        z[i] = x2 * cs[i] + x1 * sn[i];
       }
-      if (h < P.hq) {
-        uint16_t* const o = P.q_out + t * P.q_out_stride + (int64_t)h * D;
-        *reinterpret_cast<uint4*>(o + lo) = out0;
-        *reinterpret_cast<uint4*>(o + hi) = out1;
-        return;
-      }
-      const int kvh = value ? h - P.hq - P.hkv : h - P.hq;
-      const int l = value ? 16 * c : lo, r = value ? 16 * c + 8 : hi;
-      const int64_t at = row + kvh * P.cache.head_stride;
-      if constexpr (F8) {
-        uint8_t* const o = static_cast<uint8_t*>(value ? P.cache.v : P.cache.k) + at;
-        const float scale = value ? P.cache.v_scale : P.cache.k_scale;
-        *reinterpret_cast<uint2*>(o + l) = pack_e4m3(a, scale);
-        *reinterpret_cast<uint2*>(o + r) = pack_e4m3(z, scale);
-      } else {
-        uint16_t* const o = static_cast<uint16_t*>(value ? P.cache.v : P.cache.k) + at;
-        *reinterpret_cast<uint4*>(o + l) = out0;
-        *reinterpret_cast<uint4*>(o + r) = out1;
-      }
-      if (!value && P.k_out) {
-        uint16_t* const o = P.k_out + t * P.k_out_stride + (int64_t)kvh * D;
-        *reinterpret_cast<uint4*>(o + lo) = out0;
-        *reinterpret_cast<uint4*>(o + hi) = out1;
-      }
-    };
-    for (int h0 = first; h0 < heads; h0 += kBatch * step) {
-      if (h0 != first) {
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int h = h0 + i * step;
-          if (h < heads) {
-            x[i][0] = ld16(source(h, lo, false));
-            x[i][1] = ld16(source(h, hi, true));
-          }
-        }
-      }
+    }
+    v0 = pack16<BF16>(a);
+    v1 = pack16<BF16>(z);
+  };
+  // Heads h0..h1-1 of one operand, kBatch loads ahead of their use.
+  auto walk = [&](const uint16_t* src, int h0, int h1, int at0, int at1, auto put) {
+    for (int h = h0; h < h1; h += kBatch) {
+      uint4 x[kBatch][2];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i)
-        if (h0 + i * step < heads) put(h0 + i * step, x[i]);
+        if (h + i < h1) {
+          x[i][0] = ld16(src + (h + i) * D + at0);
+          x[i][1] = ld16(src + (h + i) * D + at1);
+        }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (h + i < h1) put(h + i, x[i][0], x[i][1]);
     }
-  }
+  };
+  uint16_t* const q_out = P.q_out + t * P.q_out_stride;
+  walk(P.q + t * P.q_stride, first, min(last, P.hq), lo, hi, [&](int h, uint4 v0, uint4 v1) {
+    float a[8], z[8];
+    if (turned) turn(v0, v1, a, z);
+    *reinterpret_cast<uint4*>(q_out + h * D + lo) = v0;
+    *reinterpret_cast<uint4*>(q_out + h * D + hi) = v1;
+  });
+  auto store = [&](void* pages, int h, int at0, int at1, const uint4& v0, const uint4& v1,
+                   const float (&a)[8], const float (&z)[8], float inv) {
+    const int64_t at = row + h * P.cache.head_stride;
+    if constexpr (F8) {
+      uint8_t* const o = static_cast<uint8_t*>(pages) + at;
+      *reinterpret_cast<uint2*>(o + at0) = pack_e4m3(a, inv);
+      *reinterpret_cast<uint2*>(o + at1) = pack_e4m3(z, inv);
+    } else {
+      uint16_t* const o = static_cast<uint16_t*>(pages) + at;
+      *reinterpret_cast<uint4*>(o + at0) = v0;
+      *reinterpret_cast<uint4*>(o + at1) = v1;
+    }
+  };
+  walk(P.k + t * P.k_stride, max(0, first - P.hq), min(last - P.hq, P.hkv), lo, hi,
+       [&](int h, uint4 v0, uint4 v1) {
+         float a[8], z[8];
+         if (turned) {
+           turn(v0, v1, a, z);
+         } else if (F8) {
+           unpack16<BF16>(v0, a);
+           unpack16<BF16>(v1, z);
+         }
+         store(P.cache.k, h, lo, hi, v0, v1, a, z, P.k_inv);
+         if (P.k_out) {
+           uint16_t* const o = P.k_out + t * P.k_out_stride + h * D;
+           *reinterpret_cast<uint4*>(o + lo) = v0;
+           *reinterpret_cast<uint4*>(o + hi) = v1;
+         }
+       });
+  walk(P.v + t * P.v_stride, max(0, first - P.hq - P.hkv), last - P.hq - P.hkv, 16 * c, 16 * c + 8,
+       [&](int h, uint4 v0, uint4 v1) {
+         float a[8], z[8];
+         if (F8) {
+           unpack16<BF16>(v0, a);
+           unpack16<BF16>(v1, z);
+         }
+         store(P.cache.v, h, 16 * c, 16 * c + 8, v0, v1, a, z, P.v_inv);
+       });
 }
 
 using AppendFn = void (*)(const AppendParams);
@@ -333,17 +327,15 @@ extern "C" fmha_status_t fmha_rope_append(const fmha_rope_append_args_t* args,
   P.rot = A.rotary_dim;
   P.max_position = A.max_position;
   P.err = dev.err;
-  // A block per token while they fit side by side; with few tokens the heads
-  // of each are dealt to several blocks.
-  const int slots = kAppendThreads / (d / 16);
-  const int heads = hq + 2 * hkv;
-  const int resident = dev.sms * 6;
-  const int gx = A.total_tokens < resident ? A.total_tokens : resident;
-  int gy = 1;
-  const int most = (heads + slots - 1) / slots;
-  while (gy < most && gx * gy * 2 <= resident) ++gy;
+  const int chunks = d / 16, heads = hq + 2 * hkv;
+  const int64_t threads = (int64_t)A.total_tokens * chunks;
+  P.split = (int)(kSpread / threads < 1 ? 1 : kSpread / threads > heads ? heads : kSpread / threads);
+  P.k_inv = 1.0f / P.cache.k_scale;
+  P.v_inv = 1.0f / P.cache.v_scale;
+  const int64_t blocks = (threads * P.split + kAppendThreads - 1) / kAppendThreads;
+  if (blocks > 0x7fffffff) return FMHA_ERR_UNSUPPORTED;
   return launch_serving(append_fn(A.dtype == FMHA_DTYPE_BF16, P.cache.dtype == FMHA_DTYPE_E4M3,
                                   A.interleaved != 0, d),
-                        dim3(gx, gy), kAppendThreads, 0, reinterpret_cast<cudaStream_t>(stream),
+                        dim3((unsigned)blocks), kAppendThreads, 0, reinterpret_cast<cudaStream_t>(stream),
                         P);
 }

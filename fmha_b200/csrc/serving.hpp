@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <cfloat>
 #include <cmath>
 #include <cstdlib>
 
@@ -63,7 +64,8 @@ inline fmha_status_t check_cache(const fmha_paged_cache_t& in, int hkv, int d, i
   if (c.num_pages == 1) c.page_stride = 0;
   if (c.page_stride < 0 || c.head_stride < d || c.token_stride < d || c.table_stride < 0)
     return FMHA_ERR_INVALID_ARG;
-  if (!(c.k_scale > 0.0f) || !(c.v_scale > 0.0f) || std::isinf(c.k_scale) || std::isinf(c.v_scale))
+  // Positive, finite, and with a finite reciprocal.
+  if (!(c.k_scale >= FLT_MIN) || !(c.v_scale >= FLT_MIN) || std::isinf(c.k_scale) || std::isinf(c.v_scale))
     return FMHA_ERR_INVALID_ARG;
   if (c.dtype != FMHA_DTYPE_E4M3 && (c.k_scale != 1.0f || c.v_scale != 1.0f))
     return FMHA_ERR_INVALID_ARG;

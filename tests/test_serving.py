@@ -64,7 +64,7 @@ PAGES = [({"pages_" + n: x for n, x in kw.items()}, status) for kw, status in [
     (dict(token_stride=64), INVALID), (dict(token_stride=132), MISALIGNED),
     (dict(dtype=E4M3, token_stride=136), MISALIGNED), (dict(k_scale=0.5), INVALID),
     (dict(dtype=E4M3, k_scale=0.0), INVALID), (dict(dtype=E4M3, v_scale=-1.0), INVALID),
-    (dict(dtype=E4M3, v_scale=NAN), INVALID), (dict(dtype=E4M3, k_scale=INF), INVALID),
+    (dict(dtype=E4M3, v_scale=1e-40), INVALID), (dict(dtype=E4M3, v_scale=NAN), INVALID), (dict(dtype=E4M3, k_scale=INF), INVALID),
     (dict(table_stride=-1), INVALID),
 ]]
 
