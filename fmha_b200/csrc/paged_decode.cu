@@ -58,6 +58,7 @@ namespace {
 
 constexpr int kMaxCtas = 160;      // parts the work is dealt into, at most
 constexpr int kMaxRows = 16;       // query heads of a unit
+constexpr int kMaxTokens = 0x7fffffff - 63;
 constexpr int kWholeTokens = 512;  // units up to this length are not split
 constexpr int kJoinThreads = 256;  // of the joining kernel
 
@@ -127,11 +128,17 @@ struct Place {  // a tile of a unit; units are numbered sequence by sequence
   int tile;
 };
 
+// The longest sequence: what the block table has room for, and short enough
+// for token numbers of whole tiles to stay in 32 bits.
+__device__ __forceinline__ int longest(const DecodeParams& P) {
+  const int64_t room = (int64_t)P.cache.max_pages * P.cache.page_size;
+  return room < kMaxTokens ? (int)room : kMaxTokens;
+}
+
 template <int TILE>
 __device__ __forceinline__ int tiles_of(const DecodeParams& P, int b) {
   const int n = P.cache.seqlens_kv[b];
-  const int64_t most = (int64_t)P.cache.max_pages * P.cache.page_size;
-  if (n <= 0 || n > most) return 1;  // an empty one writes its zeros, an impossible one is reported
+  if (n <= 0 || n > longest(P)) return 1;  // an empty one writes its zeros, an impossible one is reported
   return (n - 1) / TILE + 1;
 }
 
@@ -255,8 +262,7 @@ __global__ void __launch_bounds__((DecodeShape<D, F8, WIDE>::kThreads), 1)
   // A unit's length (-1: impossible) and tiles.
   auto measure = [&](int b, int& len, int& tiles) {
     const int n = P.cache.seqlens_kv[b];
-    const int64_t most = (int64_t)P.cache.max_pages * P.cache.page_size;
-    len = n >= 0 && n <= most ? n : -1;
+    len = n >= 0 && n <= longest(P) ? n : -1;
     tiles = len > 0 ? (len - 1) / S::kTile + 1 : 1;
   };
 
@@ -831,10 +837,10 @@ extern "C" fmha_status_t fmha_paged_decode(const fmha_paged_decode_args_t* args,
   if (reinterpret_cast<uintptr_t>(A.lse) & 3u) return FMHA_ERR_MISALIGNED;
   P.g = A.num_heads_q / A.num_heads_kv;
   unit_rows(P.g, &P.rows, &P.chunks);
-  const int64_t longest = (int64_t)P.cache.max_pages * P.cache.page_size;  // tokens
-  P.whole = takes_whole_units(longest);
+  const int64_t room = (int64_t)P.cache.max_pages * P.cache.page_size;  // tokens of a sequence
+  P.whole = takes_whole_units(room);
   if (!P.whole) {
-    if (!A.workspace || A.workspace_bytes < workspace_bytes_for(P.rows, d, longest))
+    if (!A.workspace || A.workspace_bytes < workspace_bytes_for(P.rows, d, room))
       return FMHA_ERR_INVALID_ARG;
     if (!aligned16(A.workspace)) return FMHA_ERR_MISALIGNED;
   }

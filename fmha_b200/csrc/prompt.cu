@@ -67,6 +67,7 @@ struct PromptParams {
   float scale_log2;
   int causal;
   int pack_log2;  // PACK
+  unsigned long long wait_ns;  // bound on every wait
   unsigned int* err;
 };
 
@@ -404,7 +405,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
   const uint32_t ring = sq + S::kQBytes;
   const int tokens = kTileRows >> P.pack_log2;  // of a tile
   auto wait = [&](int b, uint32_t parity) {  // one thread
-    return mbar_wait(bar(b), parity, &abort_flag, P.err, kWaitTimeoutNs, kSitePromptWait);
+    return mbar_wait(bar(b), parity, &abort_flag, P.err, P.wait_ns, kSitePromptWait);
   };
   auto wait_warp = [&](int b, uint32_t parity) {  // a whole warp, of one mind
     return __all_sync(kFullMask, wait(b, parity)) != 0;
@@ -1008,6 +1009,9 @@ extern "C" fmha_status_t fmha_prompt(const fmha_prompt_args_t* args, fmha_stream
   P.scale_log2 = (float)(1.4426950408889634 * scale);
   P.causal = A.causal != 0;
   P.err = dev.err;
+  // A wait lasts a piece at most: 15 ns a key on the tensor cores, and up to
+  // 5 us a key where a warp computes all its 32 rows again.
+  P.wait_ns = kWaitTimeoutNs + 20000ull * (A.total_kv < 30000000 ? A.total_kv : 30000000);
   const bool bf16 = A.dtype == FMHA_DTYPE_BF16;
   const int g = hq / hkv;
   while (P.pack_log2 < 7 && (g >> P.pack_log2) % 2 == 0) ++P.pack_log2;

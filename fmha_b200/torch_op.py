@@ -1,4 +1,6 @@
-"""PyTorch custom op over the C ABI: ``torch.ops.fmha_b200.decode``.
+"""PyTorch custom ops over the C ABI: ``torch.ops.fmha_b200.decode``, and the
+paged-cache calls ``rope_append``, ``paged_decode`` and ``prompt`` (serving.py)
+with fp16 outputs.
 
 ``decode(q, k, v) -> o`` with q [B,Hq,1,D] bf16, k/v [B,Hkv,S,D] bf16 (CUDA,
 contiguous), o [B,Hq,1,D] fp16, scale 1/sqrt(D) -- the same call as
@@ -10,7 +12,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _lib, fmha_forward_ptr
+from . import _lib, fmha_forward_ptr, serving
 
 _lib.load()
 
@@ -32,3 +34,47 @@ def decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
 @decode.register_fake
 def _(q, k, v):
     return q.new_empty((q.shape[0], q.shape[1], 1, q.shape[3]), dtype=torch.float16)
+
+
+@torch.library.custom_op("fmha_b200::rope_append", mutates_args=("k_pages", "v_pages"))
+def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
+                v_pages: torch.Tensor, block_table: torch.Tensor, seqlens_kv: torch.Tensor,
+                cos: torch.Tensor, sin: torch.Tensor, cu_seqlens_q: torch.Tensor | None = None,
+                interleaved: bool = False, k_scale: float = 1.0,
+                v_scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """(rotated q, rotated k); the pages take the new rows."""
+    return serving.fmha_rope_append(q, k, v, k_pages, v_pages, block_table, seqlens_kv, cos, sin,
+                                    cu_seqlens_q=cu_seqlens_q, interleaved=interleaved,
+                                    k_scale=k_scale, v_scale=v_scale, return_k=True)
+
+
+@rope_append.register_fake
+def _(q, k, v, k_pages, v_pages, block_table, seqlens_kv, cos, sin, cu_seqlens_q=None,
+      interleaved=False, k_scale=1.0, v_scale=1.0):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.custom_op("fmha_b200::paged_decode", mutates_args=())
+def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                 block_table: torch.Tensor, seqlens_kv: torch.Tensor, softmax_scale: float = 0.0,
+                 k_scale: float = 1.0, v_scale: float = 1.0) -> torch.Tensor:
+    return serving.fmha_paged_decode(q, k_pages, v_pages, block_table, seqlens_kv,
+                                     softmax_scale=softmax_scale, k_scale=k_scale, v_scale=v_scale)
+
+
+@paged_decode.register_fake
+def _(q, k_pages, v_pages, block_table, seqlens_kv, softmax_scale=0.0, k_scale=1.0, v_scale=1.0):
+    return q.new_empty(q.shape, dtype=torch.float16)
+
+
+@torch.library.custom_op("fmha_b200::prompt", mutates_args=())
+def prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
+           cu_seqlens_kv: torch.Tensor | None = None, causal: bool = True,
+           softmax_scale: float = 0.0) -> torch.Tensor:
+    return serving.fmha_prompt(q, k, v, cu_seqlens_q, cu_seqlens_kv, causal=causal,
+                               softmax_scale=softmax_scale)
+
+
+@prompt.register_fake
+def _(q, k, v, cu_seqlens_q, cu_seqlens_kv=None, causal=True, softmax_scale=0.0):
+    return q.new_empty(q.shape, dtype=torch.float16)

@@ -283,7 +283,8 @@ int64_t fmha_paged_decode_workspace(int num_heads_q, int num_heads_kv, int head_
  * workspace: at least fmha_paged_decode_workspace(...) bytes (null if that is
  * 0), 16-byte aligned, overwritten; calls that may run at the same time (two streams, two
  * captured graphs) need one each. It holds nothing between calls. The launch
- * depends on no length, so a captured call may be replayed as sequences grow.
+ * depends on no length, so a captured call may be replayed as sequences grow
+ * (to 2^31 - 64 tokens).
  */
 typedef struct fmha_paged_decode_args {
   const void* q;

@@ -323,16 +323,37 @@ def test_decode_offsets_past_32_bits(cuda):
     check_decode(q, pool, pool, table, lens, 1.0, 1.0, d ** -0.5, o)
 
 
+def test_decode_longest_sequence(cuda):
+    """Lengths up to the last token number are taken or refused, never read out of range: one
+    page stands in every place of the table."""
+    size, cols = 1 << 20, 2048
+    pool = torch.ones((1, 1, size, 128), dtype=BF16, device="cuda")
+    table = torch.zeros((2, cols), dtype=torch.int32, device="cuda")
+    q = randn((2, 1, 128), gen(10), BF16)
+    o = torch.full((2, 1, 128), 7.0, dtype=FP16, device="cuda")
+    for n in (2 ** 31 - 1, 2 ** 31 - 63):
+        fmha_b200.fmha_paged_decode(q, pool, pool, table, i32([n, 3]), o=o)
+        torch.cuda.synchronize()
+        assert error_site() == (fmha_b200.FMHA_ERR_INVALID_ARG, SITE_DECODE_LENGTH)
+        assert bool((o[0] == 7.0).all()) and bool((o[1] == 1.0).all())
+    fmha_b200.fmha_paged_decode(q, pool, pool, table, i32([3 * size + 17, 3]), o=o)
+    torch.cuda.synchronize()
+    assert fmha_b200.device_error() == 0
+    assert bool((o - 1.0).abs().max() <= 2.0 ** -10)
+
+
 @pytest.mark.parametrize("columns", [None, 100])
-@pytest.mark.parametrize("d,ctype", [(128, BF16), (256, BF16), (128, E4M3)])
-def test_decode_nonfinite(cuda, d, ctype, columns):
+@pytest.mark.parametrize("d,ctype,gq", [(128, BF16, 2), (256, BF16, 2), (128, E4M3, 2), (128, FP16, 3),
+                                        (128, BF16, 16), (256, FP16, 12)])
+def test_decode_nonfinite(cuda, d, ctype, gq, columns):
     """NaN and infinities in keys, values and queries reach exactly the rows and columns that
     the formula takes them to."""
     g = gen(11)
-    lens, hkv, gq, size = [40, 40, 40, 40, 40, 0], 2, 2, 16
+    lens, hkv, size = [40, 40, 40, 40, 40, 0], 2, 16
+    dtype = BF16 if ctype == E4M3 else ctype
     table, pages = make_table(lens, size, g, columns=columns)
-    pk, pv = make_pool(pages, hkv, size, d, BF16, g), make_pool(pages, hkv, size, d, BF16, g)
-    q = randn((6, hkv * gq, d), g, BF16)
+    pk, pv = make_pool(pages, hkv, size, d, dtype, g), make_pool(pages, hkv, size, d, dtype, g)
+    q = randn((6, hkv * gq, d), g, dtype)
     at = lambda b, j: (int(table[b, j // size]), j % size)  # noqa: E731
     p, r = at(0, 39)
     pk[p, 0, r, 3] = float("nan")                       # a NaN score
@@ -359,7 +380,7 @@ def test_decode_nonfinite(cuda, d, ctype, columns):
     if ctype == E4M3:
         bad[1, gq:, 7] = True
     else:
-        bad[4, :2] = True
+        bad[4, :gq] = True  # the other queries meet -inf in every key too
         assert bool(torch.isinf(o[1, gq:, 7]).all())
     assert torch.equal(torch.isnan(o), bad)
     assert bool((o[5] == 0).all())
@@ -490,6 +511,7 @@ def prompt_case(nq, nk, hq, hkv, d, dtype, out, causal, seed, scale=0.0, pad=5):
     (2, 2, 128, BF16, FP16, True), (8, 2, 128, BF16, BF16, True), (6, 2, 128, FP16, FP16, False),
     (5, 1, 128, FP16, BF16, True), (16, 1, 128, BF16, BF16, False), (4, 2, 256, BF16, BF16, True),
     (8, 1, 256, FP16, FP16, True), (3, 1, 256, BF16, FP16, False), (32, 1, 128, BF16, FP16, True),
+    (64, 1, 256, BF16, BF16, True), (128, 1, 128, BF16, BF16, True), (256, 1, 128, FP16, FP16, True),
 ])
 def test_prompt(cuda, nq, hq, hkv, d, dtype, out, causal):
     prompt_case(nq, nq, hq, hkv, d, dtype, out, causal, seed=sum(nq) + hq)
@@ -507,6 +529,13 @@ def test_prompt_with_other_keys_than_queries(cuda, nq, nk, hq, hkv, d, dtype, ou
 @pytest.mark.parametrize("d,dtype,out", [(128, BF16, BF16), (256, FP16, FP16), (128, BF16, FP16)])
 def test_prompt_long(cuda, d, dtype, out):
     prompt_case([2500, 1], [2500, 4000], 4, 2, d, dtype, out, True, seed=d)
+
+
+@pytest.mark.parametrize("b", [300, 40])
+def test_prompt_many_sequences(cuda, b):
+    """More sequences than the planning warp sorts, empty ones among them."""
+    nq = [(7 * i) % 23 if i % 11 else 140 + i for i in range(b)]
+    prompt_case(nq, [n + i % 3 for i, n in enumerate(nq)], 4, 2, 128, BF16, BF16, True, seed=b)
 
 
 def test_prompt_large_scores(cuda):
@@ -625,3 +654,24 @@ def test_serving_run(cuda, ctype):
             check_decode(q, pk, pv, table, lens.tolist(), ks, vs, d ** -0.5, o)
         new = [1] * b
     assert fmha_b200.device_error() == 0
+
+
+def test_torch_ops(cuda):
+    """torch.ops.fmha_b200.{rope_append,paged_decode,prompt} make the same calls."""
+    import fmha_b200.torch_op  # noqa: F401
+    g = gen(33)
+    ops = torch.ops.fmha_b200
+    new, hq, hkv, d, size = [5, 20], 4, 2, 128, 16
+    table, pages = make_table(new, size, g)
+    pools = [torch.zeros((pages, hkv, size, d), dtype=BF16, device="cuda") for _ in range(4)]
+    q, k, v = (randn((25, h, d), g, BF16) for h in (hq, hkv, hkv))
+    cos, sin = angles(32, d, g)
+    lens, cu = i32(new), starts(new)
+    a = ops.rope_append(q, k, v, pools[0], pools[1], table, lens, cos, sin, cu)
+    b = fmha_b200.fmha_rope_append(q, k, v, pools[2], pools[3], table, lens, cos, sin, cu_seqlens_q=cu, return_k=True)
+    for x, y in ((a[0], b[0]), (a[1], b[1]), (pools[0], pools[2]), (pools[1], pools[3])):
+        assert torch.equal(bits(x), bits(y))
+    assert torch.equal(ops.prompt(a[0], a[1], v, cu), fmha_b200.fmha_prompt(a[0], a[1], v, cu))
+    q1 = a[0][:2].contiguous()
+    assert torch.equal(ops.paged_decode(q1, pools[0], pools[1], table, lens),
+                       fmha_b200.fmha_paged_decode(q1, pools[0], pools[1], table, lens))
