@@ -6,7 +6,6 @@ from __future__ import annotations
 
 import ctypes
 import os
-import struct
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "libfmha_b200.so")
@@ -60,18 +59,6 @@ class PromptArgs(ctypes.Structure):
                [(n, _i) for n in ("total_q", "total_kv", "batch", "num_heads_q", "num_heads_kv",
                                   "head_dim", "causal", "dtype", "o_dtype")] + \
                [("softmax_scale", _f)]
-
-
-def packer(cls):
-    """The bytes of an argument struct from its values in order (nested structs' values in
-    place), several times faster than filling the ctypes object."""
-    codes = {_vp: "P", _i64: "q", _i: "i", _f: "f"}
-
-    def walk(c):
-        return "".join(walk(t) if issubclass(t, ctypes.Structure) else codes[t] for _, t in c._fields_)
-    s = struct.Struct("@" + walk(cls) + "0q")
-    assert s.size == ctypes.sizeof(cls)
-    return s.pack
 
 
 # Every symbol include/fmha.h declares, with (restype, argtypes).

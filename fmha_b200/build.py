@@ -4,6 +4,8 @@
   sm_100a only: the decode_*.cu kernels compiled once per head_dim, plus
   fmha_api.cu, fmha_noalloc.cu and the paged-cache operators (rope_append.cu,
   paged_decode.cu, prompt.cu);
+* ``fmha_b200/_serving.so`` -- the Python module behind serving.py
+  (serving_py.cpp; torch's headers, no kernels);
 * ``fmha_b200/bin/fmha_host`` -- the C++ benchmark/validation host linked
   against that library (when its source is present).
 
@@ -23,6 +25,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libfmha_b200.so")
+BINDING = os.path.join(PKG, "_serving.so")
 HOST_BIN = os.path.join(PKG, "bin", "fmha_host")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -91,6 +94,28 @@ def build_lib(force: bool = False, verbose: bool = False) -> str:
     return LIB
 
 
+def build_binding(force: bool = False) -> str:
+    import sysconfig
+
+    import torch
+    src = os.path.join(CSRC, "serving_py.cpp")
+    base = os.path.dirname(torch.__file__)
+    deps = [src, os.path.join(ROOT, "include", "fmha.h"), os.path.join(base, "version.py")]
+    if force or _stale(BINDING, deps):
+        cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               "-I" + os.path.join(base, "include"),
+               "-I" + os.path.join(base, "include", "torch", "csrc", "api", "include"),
+               "-I" + cuda, "-I" + sysconfig.get_paths()["include"], src, "-o", BINDING,
+               "-L" + os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
+               "-lc10_cuda"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"g++ failed for serving_py.cpp:\n{r.stdout}\n{r.stderr}")
+    return BINDING
+
+
 def build_host(force: bool = False) -> str | None:
     src = os.path.join(CSRC, "fmha_host.cpp")
     if not os.path.exists(src):
@@ -106,6 +131,7 @@ def build_host(force: bool = False) -> str | None:
 
 def build(force: bool = False, verbose: bool = False) -> None:
     build_lib(force, verbose)
+    build_binding(force)
     build_host(force)
 
 
