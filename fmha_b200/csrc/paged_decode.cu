@@ -236,24 +236,32 @@ __global__ void __launch_bounds__((DecodeShape<D, F8, WIDE>::kThreads), 1)
     const int units = P.batch * HU;
     const int u0 = P.whole ? (int)((int64_t)units * blockIdx.x / gridDim.x) : 0;
     const int u1 = P.whole ? (int)((int64_t)units * (blockIdx.x + 1) / gridDim.x) : units;
-    WorkList<S::kTile, S::kThreads> list{P, HU, u0, u1,
-                                         reinterpret_cast<int64_t*>(smem), 0, 0};  // no ring yet
-    const int64_t total = list.sum(warp_sum);
-    int64_t lo = 0;
-    hi_at = total;
-    if (!P.whole) {
-      per = total <= 0x7fffffff ? (int64_t)(((uint32_t)total + gridDim.x - 1) / gridDim.x)
-                                : (total + gridDim.x - 1) / gridDim.x;
-      if (per < kW) per = kW;
-      lo = min(total, per * blockIdx.x);
-      hi_at = min(total, lo + per);
-      if (threadIdx.x == 0) P.part_unit[blockIdx.x] = make_int2(-1, 0);
-    }
-    if (threadIdx.x <= kW) {
-      const int64_t mine = hi_at - lo;
-      const int w = threadIdx.x;
-      range[w] = list.locate(
-          lo + (mine <= 0x0fffffff ? (int64_t)((uint32_t)mine * w / kW) : mine * w / kW), total);
+    if (P.whole && u1 - u0 == 1) {  // one unit: nothing to add up
+      if (threadIdx.x <= kW) {
+        const int w = threadIdx.x, n = tiles_of<S::kTile>(P, u0 / HU), at = (n + 1) * w / kW;
+        range[w] = at >= n ? Place{u1, 0} : Place{u0, at};
+      }
+      hi_at = 0;  // no unit goes on in another CTA
+    } else {
+      WorkList<S::kTile, S::kThreads> list{P, HU, u0, u1,
+                                           reinterpret_cast<int64_t*>(smem), 0, 0};  // no ring yet
+      const int64_t total = list.sum(warp_sum);
+      int64_t lo = 0;
+      hi_at = total;
+      if (!P.whole) {
+        per = total <= 0x7fffffff ? (int64_t)(((uint32_t)total + gridDim.x - 1) / gridDim.x)
+                                  : (total + gridDim.x - 1) / gridDim.x;
+        if (per < kW) per = kW;
+        lo = min(total, per * blockIdx.x);
+        hi_at = min(total, lo + per);
+        if (threadIdx.x == 0) P.part_unit[blockIdx.x] = make_int2(-1, 0);
+      }
+      if (threadIdx.x <= kW) {
+        const int64_t mine = hi_at - lo;
+        const int w = threadIdx.x;
+        range[w] = list.locate(
+            lo + (mine <= 0x0fffffff ? (int64_t)((uint32_t)mine * w / kW) : mine * w / kW), total);
+      }
     }
   }
   __syncthreads();

@@ -382,6 +382,9 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
   }
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](int i) { return bar0 + 8 * i; };
+  const int tokens = kTileRows >> P.pack_log2;  // of a tile
+  WorkList list;
+  if (warp == S::kPlanWarp) list.load(P, kTiles * tokens);
   if (warp == S::kMmaWarp) {
     if (lane == 0) {
       abort_flag = 0;
@@ -403,7 +406,6 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
   const uint32_t tmem = tmem_slot;
   const uint32_t sq = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t ring = sq + S::kQBytes;
-  const int tokens = kTileRows >> P.pack_log2;  // of a tile
   auto wait = [&](int b, uint32_t parity) {  // one thread
     return mbar_wait(bar(b), parity, &abort_flag, P.err, P.wait_ns, kSitePromptWait);
   };
@@ -608,8 +610,6 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
       // started, until there are none.
       int index = blockIdx.x, asked = 0;
       bool ok = true;
-      WorkList list;
-      list.load(P, kTiles * tokens);
       while (ok) {
         if (lane == 0 && index >= 0) {
           fence_async_shared();  // the last answer has been read
