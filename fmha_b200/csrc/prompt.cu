@@ -355,7 +355,8 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
     kPMost = kSFull + 2,  // of all keys but 32..63
     kPFull = kPMost + 2,
     kODone = kPFull + 2,
-    kOFree = kODone + 2,
+    kPVDone = kODone + 2,  // every P.V, at head_dim 256
+    kOFree = kPVDone + 1,
     kWorkFull = kOFree + 2,
     kWorkFree = kWorkFull + 2,
     kAnswer = kWorkFree + 2,
@@ -444,7 +445,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
     const uint32_t o_at = lanes + S::kColO + (kTiles == 2 ? 128 * tile : 0);
     const float sc = P.scale_log2;
     int block = 0;    // key blocks so far, of this tile
-    int outputs = 0;  // and outputs (head_dim 128)
+    int outputs = 0;  // and outputs
     bool ok = true;
     while (ok && next_work()) {
       const int n = tile ? w.n1 : w.n0;
@@ -511,7 +512,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
           if (j > 0) {
             // The scores of block j follow P.V of block j-1 (head_dim 128), or of j-2 (256).
             if (kTiles == 1) {
-              ok = wait_warp(kODone, (block - 1) & 1);
+              ok = wait_warp(kPVDone, (block - 1) & 1);
               if (!ok) break;
               tmem_fence_after();
             }
@@ -569,14 +570,8 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
       }
 
       if (ok && n > 0) {
-        if (kTiles == 2) {
-          ok = wait_warp(kODone + tile, outputs & 1);
-          ++outputs;
-        } else {
-          // One phase after the other: the last but one may still be open.
-          if (n > 1) ok = wait_warp(kODone, (block - 2) & 1);
-          ok = ok && wait_warp(kODone, (block - 1) & 1);
-        }
+        ok = wait_warp(kODone + tile, outputs & 1);
+        ++outputs;
         tmem_fence_after();
       }
       if (!ok) break;
@@ -868,7 +863,8 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
                 pv(S::kColO + 128 * h, 128 * buf, v, false, false);
                 done();
               }
-              if (ok) umma_commit(bar(kODone));
+              if (ok) umma_commit(bar(kPVDone));
+              if (ok && j + 1 == blocks) umma_commit(bar(kODone));
             }
           }
         }

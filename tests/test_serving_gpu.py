@@ -538,6 +538,36 @@ def test_prompt_many_sequences(cuda, b):
     prompt_case(nq, [n + i % 3 for i, n in enumerate(nq)], 4, 2, 128, BF16, BF16, True, seed=b)
 
 
+@pytest.mark.parametrize("d,dtype,out", [(128, BF16, BF16), (128, BF16, FP16), (256, FP16, FP16), (256, BF16, BF16)])
+def test_prompt_repeats(cuda, d, dtype, out):
+    """Many short and long pieces in a row, on and on: the same bits every time, and no wait
+    that runs out."""
+    g = gen(d)
+    nq = [1, 700, 33, 128, 5, 260, 64, 1025, 17] * 8
+    q, k, v = (randn((sum(nq), h, d), g, dtype) for h in (8, 2, 2))
+    cu = starts(nq)
+    first = fmha_b200.fmha_prompt(q, k, v, cu, out_dtype=out)
+    for _ in range(150):
+        o = fmha_b200.fmha_prompt(q, k, v, cu, out_dtype=out)
+    torch.cuda.synchronize()
+    assert fmha_b200.device_error() == 0
+    assert torch.equal(bits(o), bits(first))
+
+
+def test_decode_repeats(cuda):
+    g = gen(41)
+    lens = [1, 700, 33, 0, 5000, 260, 64, 1025, 17] * 6
+    table, pages = make_table(lens, 16, g)
+    pk, pv = make_pool(pages, 2, 16, 128, BF16, g), make_pool(pages, 2, 16, 128, BF16, g)
+    q, n = randn((len(lens), 8, 128), g, BF16), i32(lens)
+    first = fmha_b200.fmha_paged_decode(q, pk, pv, table, n)
+    for _ in range(150):
+        o = fmha_b200.fmha_paged_decode(q, pk, pv, table, n)
+    torch.cuda.synchronize()
+    assert fmha_b200.device_error() == 0
+    assert torch.equal(bits(o), bits(first))
+
+
 def test_prompt_large_scores(cuda):
     """Scores of hundreds: the running maximum rises late and far, weights underflow."""
     g = gen(21)
