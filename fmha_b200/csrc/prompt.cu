@@ -360,6 +360,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
     kWorkFull = kOFree + 2,
     kWorkFree = kWorkFull + 2,
     kAnswer = kWorkFree + 2,
+    kClaim,  // the piece at hand is about to end
     kTrimGo,
     kTrimmed,
     kDrain,
@@ -602,15 +603,13 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
     if (warp == S::kPlanWarp) {
       // ---------------------------------------------------------- work list
       // This block's own piece first, then those of blocks that have not
-      // started, until there are none.
-      int index = blockIdx.x, asked = 0;
+      // started, until there are none. A block is claimed when the last piece
+      // has three key blocks to go: early enough to hide the claim, and late
+      // enough that the blocks with the least work left take the most (claims
+      // at a piece's start: 92 us instead of 73 on 4096 tokens, 16/4 heads).
+      int index = blockIdx.x, asked = 0, claims = 0;
       bool ok = true;
       while (ok) {
-        if (lane == 0 && index >= 0) {
-          fence_async_shared();  // the last answer has been read
-          mbar_arrive_expect_tx(bar(kAnswer), 16);
-          clc_try_cancel(smem_u32(&answer), bar(kAnswer));
-        }
         Work mine;
         const bool found = index >= 0 && list.find(P, index, kTiles * tokens, &mine);
         if (found || index < 0) {
@@ -626,13 +625,19 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
             mbar_arrive(bar(kWorkFull + s));
           }
           ++piece;
+          if (index < 0 || !ok) break;
+          ok = wait_warp(kClaim, claims & 1);
+          ++claims;
+          if (!ok) break;
         }
-        if (index < 0) break;
-        // The answer is always waited for, so that it lands while the block is there.
-        const bool got = wait_warp(kAnswer, asked & 1);
-        ok = ok && got;
+        if (lane == 0) {
+          fence_async_shared();  // the last answer has been read
+          mbar_arrive_expect_tx(bar(kAnswer), 16);
+          clc_try_cancel(smem_u32(&answer), bar(kAnswer));
+        }
+        ok = wait_warp(kAnswer, asked & 1);
         ++asked;
-        if (got) index = clc_granted(smem_u32(&answer));
+        if (ok) index = clc_granted(smem_u32(&answer));
         __syncwarp();
       }
     } else if (warp == S::kTmaWarp) {
@@ -773,7 +778,10 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
         };
         while (ok && next_work_one()) {
           const int blocks = max(w.n0, w.n1);
-          if (blocks <= 0) continue;
+          if (blocks <= 0) {
+            mbar_arrive(bar(kClaim));
+            continue;
+          }
           ok = wait(kQFull, loaded & 1);
           ++loaded;
           if constexpr (kTiles == 2) {
@@ -792,6 +800,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
               if (blocks == 1) umma_commit(bar(kQFree));
             }
             for (int j = 0; j < blocks && ok; ++j) {
+              if (j == max(0, blocks - 3)) mbar_arrive(bar(kClaim));
               const uint32_t v = take();
               if (!ok) break;
               const int v_slot = slot;
@@ -849,6 +858,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
             };
             if (ok) scores(0);
             for (int j = 0; j < blocks && ok; ++j) {
+              if (j == max(0, blocks - 3)) mbar_arrive(bar(kClaim));
               if (j + 1 < blocks) scores(j + 1);
               const int buf = fed0 & 1;
               weights(buf, fed0 >> 1, 0, out0, j == 0);
