@@ -456,8 +456,8 @@ __global__ void __launch_bounds__((DecodeShape<D, F8, WIDE>::kThreads), 1)
             for (int n = 0; n < 2; ++n)
 #pragma unroll
               for (int j = 0; j < 2; ++j) {
-                const uint32_t x = w[2 * n + j];
-                const uint32_t b0 = e4m3x2_to_half2(x & 0xffffu), b1 = e4m3x2_to_half2(x >> 16);
+                uint32_t b0, b1;
+                e4m3x4_to_half2(w[2 * n + j], b0, b1);
                 if constexpr (WIDE)
                   mma16<kB>(sc[2 * u + n], qa[s + j][0], qa[s + j][1], qa[s + j][2], qa[s + j][3], b0, b1);
                 else
@@ -547,11 +547,11 @@ __global__ void __launch_bounds__((DecodeShape<D, F8, WIDE>::kThreads), 1)
             if constexpr (F8) {
               // Each 32-bit word: two tokens x two adjacent columns; tile 2k
               // takes the even columns of a 16-byte piece, tile 2k+1 the odd.
-              const uint32_t x = w[2 * j], y = w[2 * j + 1];
-              pv(acc[2 * (i + j)], e4m3x2_to_half2(__byte_perm(x, 0, 0x4420)),
-                 e4m3x2_to_half2(__byte_perm(y, 0, 0x4420)));
-              pv(acc[2 * (i + j) + 1], e4m3x2_to_half2(__byte_perm(x, 0, 0x4431)),
-                 e4m3x2_to_half2(__byte_perm(y, 0, 0x4431)));
+              uint32_t x0, x1, y0, y1;
+              e4m3x4_to_half2(__byte_perm(w[2 * j], 0, 0x3120), x0, x1);
+              e4m3x4_to_half2(__byte_perm(w[2 * j + 1], 0, 0x3120), y0, y1);
+              pv(acc[2 * (i + j)], x0, y0);
+              pv(acc[2 * (i + j) + 1], x1, y1);
             } else {
               pv(acc[i + j], w[2 * j], w[2 * j + 1]);
             }

@@ -94,13 +94,12 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   lo = pack2<BF16>(fmaxf(x - h.x, kLeast), fmaxf(y - h.y, kLeast));
 }
 
-// Two e4m3 codes (low 16 bits) as two fp16 values: exact.
-__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t codes) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}"
-      : "=r"(r)
+// Four e4m3 codes as two pairs of fp16 values (low codes in `lo`): exact.
+__device__ __forceinline__ void e4m3x4_to_half2(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
       : "r"(codes));
-  return r;
 }
 
 }  // namespace fmha
