@@ -205,6 +205,66 @@ struct WorkList {
   }
 };
 
+// The same list for up to kFew sequences, by one warp without shared memory
+// or barriers: lane i has sequences 4i .. 4i+3 of it.
+constexpr int kFew = 128;
+
+template <int TILE>
+struct FewList {
+  int hu, u0, u1, b_lo;
+  int tiles[4];
+  int64_t before, total;
+
+  __device__ int first(int b) const { return max(u0, b * hu); }
+  __device__ int units(int b) const { return max(0, min(u1, (b + 1) * hu) - first(b)); }
+  __device__ void load(const DecodeParams& P, int hu_, int u0_, int u1_) {
+    hu = hu_;
+    u0 = u0_;
+    u1 = u1_;
+    const int lane = threadIdx.x & 31;
+    b_lo = u0 / hu + 4 * lane;
+    int64_t mine = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int b = b_lo + k;
+      tiles[k] = b < P.batch ? tiles_of<TILE>(P, b) : 1;
+      if (b < P.batch) mine += (int64_t)units(b) * (tiles[k] + 1);
+    }
+    int64_t inc = mine;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const int64_t y = __shfl_up_sync(kFullMask, inc, s);
+      if (lane >= s) inc += y;
+    }
+    before = inc - mine;
+    total = __shfl_sync(kFullMask, inc, 31);
+  }
+  __device__ Place locate(int64_t at) const {  // the whole warp
+    if (at >= total) return {u1, 0};
+    const int owner = 31 - __clz(__ballot_sync(kFullMask, before <= at));
+    int64_t in = at - before;  // of the owner's sequences
+    int unit = 0, tile = 0;
+    bool found = false;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int b = b_lo + k, n = tiles[k];
+      const int64_t here = (int64_t)units(b) * (n + 1);
+      if (!found && in < here) {
+        const int u = here <= 0x7fffffff ? (int)((uint32_t)in / (uint32_t)(n + 1)) : (int)(in / (n + 1));
+        tile = (int)(in - (int64_t)u * (n + 1));
+        unit = first(b) + u;
+        if (tile == n) {
+          ++unit;
+          tile = 0;
+        }
+        found = true;
+      }
+      in -= here;
+    }
+    return {__shfl_sync(kFullMask, unit, owner), __shfl_sync(kFullMask, tile, owner)};
+  }
+};
+
 // ------------------------------------------------------------ the kernel
 
 template <int D, bool BF16, bool F8, bool WIDE>
@@ -228,25 +288,18 @@ __global__ void __launch_bounds__((DecodeShape<D, F8, WIDE>::kThreads), 1)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int gr = lane >> 2, gc = lane & 3;
   const int HU = P.hkv * P.chunks;
-  if (threadIdx.x < 2 * kW) slot_unit[threadIdx.x] = -1;
+  if (lane < 2) slot_unit[2 * warp + lane] = -1;
+  __syncwarp();
 
-  // The CTA's positions [lo, hi) of the list, and its warps' places there.
-  int64_t per = 0, hi_at;
+  // The CTA's positions [lo, hi) of the list, and this warp's places there.
+  int64_t per = 0, hi_at = 0;
+  Place from, to;
   {
     const int units = P.batch * HU;
     const int u0 = P.whole ? (int)((int64_t)units * blockIdx.x / gridDim.x) : 0;
     const int u1 = P.whole ? (int)((int64_t)units * (blockIdx.x + 1) / gridDim.x) : units;
-    if (P.whole && u1 - u0 == 1) {  // one unit: nothing to add up
-      if (threadIdx.x <= kW) {
-        const int w = threadIdx.x, n = tiles_of<S::kTile>(P, u0 / HU), at = (n + 1) * w / kW;
-        range[w] = at >= n ? Place{u1, 0} : Place{u0, at};
-      }
-      hi_at = 0;  // no unit goes on in another CTA
-    } else {
-      WorkList<S::kTile, S::kThreads> list{P, HU, u0, u1,
-                                           reinterpret_cast<int64_t*>(smem), 0, 0};  // no ring yet
-      const int64_t total = list.sum(warp_sum);
-      int64_t lo = 0;
+    auto deal = [&](int64_t total, int64_t& lo) {  // the CTA's share
+      lo = 0;
       hi_at = total;
       if (!P.whole) {
         per = total <= 0x7fffffff ? (int64_t)(((uint32_t)total + gridDim.x - 1) / gridDim.x)
@@ -256,16 +309,34 @@ __global__ void __launch_bounds__((DecodeShape<D, F8, WIDE>::kThreads), 1)
         hi_at = min(total, lo + per);
         if (threadIdx.x == 0) P.part_unit[blockIdx.x] = make_int2(-1, 0);
       }
-      if (threadIdx.x <= kW) {
-        const int64_t mine = hi_at - lo;
-        const int w = threadIdx.x;
-        range[w] = list.locate(
-            lo + (mine <= 0x0fffffff ? (int64_t)((uint32_t)mine * w / kW) : mine * w / kW), total);
-      }
+    };
+    auto share = [&](int64_t lo, int w) {  // where warp w's begins
+      const int64_t mine = hi_at - lo;
+      return lo + (mine <= 0x0fffffff ? (int64_t)((uint32_t)mine * w / kW) : mine * w / kW);
+    };
+    int64_t lo;
+    if (P.whole && u1 - u0 == 1) {  // one unit: nothing to add up
+      const int n = tiles_of<S::kTile>(P, u0 / HU);
+      const int at = (n + 1) * warp / kW, next_at = (n + 1) * (warp + 1) / kW;
+      from = at >= n ? Place{u1, 0} : Place{u0, at};
+      to = next_at >= n ? Place{u1, 0} : Place{u0, next_at};
+    } else if ((P.whole ? (u1 > u0 ? (u1 - 1) / HU - u0 / HU + 1 : 0) : P.batch) <= kFew) {
+      FewList<S::kTile> list;
+      list.load(P, HU, u0, u1);
+      deal(list.total, lo);
+      from = list.locate(share(lo, warp));
+      to = list.locate(share(lo, warp + 1));
+    } else {
+      WorkList<S::kTile, S::kThreads> list{P, HU, u0, u1,
+                                           reinterpret_cast<int64_t*>(smem), 0, 0};  // no ring yet
+      const int64_t total = list.sum(warp_sum);
+      deal(total, lo);
+      if (threadIdx.x <= kW) range[threadIdx.x] = list.locate(share(lo, threadIdx.x), total);
+      __syncthreads();
+      from = range[warp];
+      to = range[warp + 1];
     }
   }
-  __syncthreads();
-  const Place from = range[warp], to = range[warp + 1];
   const int units_end = to.unit + (to.tile > 0 ? 1 : 0);  // units met here, the last maybe in part
   // A unit's length (-1: impossible) and tiles.
   auto measure = [&](int b, int& len, int& tiles) {
@@ -620,6 +691,7 @@ __global__ void __launch_bounds__((DecodeShape<D, F8, WIDE>::kThreads), 1)
     }
   }
   cp_async_wait<0>();
+  if (warp == kW - 1 && lane == 0) range[kW] = to;
   __syncthreads();
 
   // Joins the CTA's held results, unit by unit; the rows of all of them are
