@@ -242,24 +242,22 @@ struct FewList {
   __device__ Place locate(int64_t at) const {  // the whole warp
     if (at >= total) return {u1, 0};
     const int owner = 31 - __clz(__ballot_sync(kFullMask, before <= at));
-    int64_t in = at - before;  // of the owner's sequences
-    int unit = 0, tile = 0;
-    bool found = false;
+    int64_t in = at - before, here = 0;  // into the owner's sequences, and the one it falls in
+    int k = 0, n = tiles[0];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int b = b_lo + k, n = tiles[k];
-      const int64_t here = (int64_t)units(b) * (n + 1);
-      if (!found && in < here) {
-        const int u = here <= 0x7fffffff ? (int)((uint32_t)in / (uint32_t)(n + 1)) : (int)(in / (n + 1));
-        tile = (int)(in - (int64_t)u * (n + 1));
-        unit = first(b) + u;
-        if (tile == n) {
-          ++unit;
-          tile = 0;
-        }
-        found = true;
+    for (int i = 0; i < 4; ++i) {
+      if (i > 0 && k == i - 1 && in >= here) {  // on to sequence i
+        in -= here;
+        k = i;
+        n = tiles[i];
       }
-      in -= here;
+      if (k == i) here = (int64_t)units(b_lo + i) * (n + 1);
+    }
+    const int u = here <= 0x7fffffff ? (int)((uint32_t)in / (uint32_t)(n + 1)) : (int)(in / (n + 1));
+    int unit = first(b_lo + k) + u, tile = (int)(in - (int64_t)u * (n + 1));
+    if (tile == n) {
+      ++unit;
+      tile = 0;
     }
     return {__shfl_sync(kFullMask, unit, owner), __shfl_sync(kFullMask, tile, owner)};
   }
