@@ -904,7 +904,8 @@ extern "C" fmha_status_t fmha_paged_decode(const fmha_paged_decode_args_t* args,
   if (st != FMHA_OK) return st;
   if (A.dtype != FMHA_DTYPE_BF16 && A.dtype != FMHA_DTYPE_FP16) return FMHA_ERR_UNSUPPORTED;
   if (A.o_dtype != FMHA_DTYPE_BF16 && A.o_dtype != FMHA_DTYPE_FP16) return FMHA_ERR_UNSUPPORTED;
-  if (!(A.softmax_scale >= 0.0f) || std::isinf(A.softmax_scale)) return FMHA_ERR_INVALID_ARG;
+  float scale_log2;
+  if ((st = check_scale(A.softmax_scale, d, 1.0f, &scale_log2)) != FMHA_OK) return st;
   if (batch == 0) return FMHA_OK;
   if ((st = check_rows(A.q, A.q_stride, A.num_heads_q, d)) != FMHA_OK ||
       (st = check_rows(A.o, A.o_stride, A.num_heads_q, d)) != FMHA_OK)
@@ -912,6 +913,7 @@ extern "C" fmha_status_t fmha_paged_decode(const fmha_paged_decode_args_t* args,
   DecodeParams P;
   std::memset(&P, 0, sizeof(P));
   if ((st = check_cache(A.cache, A.num_heads_kv, d, A.dtype, &P.cache)) != FMHA_OK) return st;
+  if ((st = check_scale(A.softmax_scale, d, P.cache.k_scale, &P.scale_log2)) != FMHA_OK) return st;
   if (reinterpret_cast<uintptr_t>(A.lse) & 3u) return FMHA_ERR_MISALIGNED;
   P.g = A.num_heads_q / A.num_heads_kv;
   unit_rows(P.g, &P.rows, &P.chunks);
@@ -933,9 +935,6 @@ extern "C" fmha_status_t fmha_paged_decode(const fmha_paged_decode_args_t* args,
   P.hkv = A.num_heads_kv;
   P.q_stride = A.q_stride;
   P.o_stride = A.o_stride;
-  const double scale =
-      A.softmax_scale > 0.0f ? (double)A.softmax_scale : 1.0 / std::sqrt((double)d);
-  P.scale_log2 = (float)(1.4426950408889634 * scale * P.cache.k_scale);
   P.o_bf16 = A.o_dtype == FMHA_DTYPE_BF16;
   P.err = dev.err;
   int log2_up = 0;

@@ -104,15 +104,18 @@ struct Work {
 // The list of all pieces (`tokens` tokens of a sequence, of one head group).
 // Up to kSorted sequences it goes by the tokens' place, the last places
 // first: with a causal mask the longest pieces come first and the card ends
-// evenly (29 ragged prompts: 138 us in the
-// sequences' order, 113 us so). The
+// evenly (29 ragged prompts: 138 us in the sequences' order, 113 us so). The
 // planning warp keeps the sequences' piece counts, 8 to a lane. More
-// sequences go one after the other, each from its end to its start.
+// sequences go one after the other, each from its end to its start; the
+// counts are then those of kSorted groups of them, in shared memory, and a
+// piece's sequence is looked for in its group (walking over all sequences from the first took
+// 41 ms on 8192 sequences of 16 tokens).
 constexpr int kSorted = 256;
 
 struct WorkList {
   int parts[kSorted / 32];  // of sequences lane, lane + 32, ..
   int all, places;          // pieces, and the most of a sequence
+  int* groups;              // MANY: pieces of the groups, in shared memory
 
   // Pieces of sequence b; one impossible at the head of the list is reported.
   __device__ static int parts_of(const PromptParams& P, int b, int tokens) {
@@ -133,6 +136,22 @@ struct WorkList {
 #pragma unroll
     for (int k = 0; k < kSorted / 32; ++k) places = max(places, parts[k]);
     places = __reduce_max_sync(kFullMask, places);
+  }
+  __device__ static uint32_t group_of(const PromptParams& P) {  // sequences of a group
+    return 32 * (((uint32_t)P.batch + 32 * kSorted - 1) / (32 * kSorted));
+  }
+  __device__ void load_groups(const PromptParams& P, int tokens) const {  // the whole CTA
+    const uint32_t group = group_of(P), batch = P.batch;
+    for (uint32_t g = threadIdx.x >> 5; g < kSorted; g += blockDim.x >> 5) {
+      const uint32_t b0 = g * group;
+      int n = 0;
+      if (b0 < batch) {
+        for (uint32_t i = threadIdx.x & 31; i < group; i += 32)
+          if (b0 + i < batch) n += parts_of(P, b0 + i, tokens);
+        n = __reduce_add_sync(kFullMask, n);
+      }
+      if ((threadIdx.x & 31) == 0) groups[g] = n;
+    }
   }
   // Pieces at place t or later.
   __device__ int from_place(int t) const {
@@ -175,20 +194,36 @@ struct WorkList {
     }
     return false;
   }
-  __device__ static bool in_order(const PromptParams& P, int at, int tokens, int* seq, int* place) {
+  __device__ bool in_order(const PromptParams& P, int at, int tokens, int* seq, int* place) const {
     const int lane = threadIdx.x & 31;
-    for (int b0 = 0; b0 < P.batch; b0 += 32) {
-      const int n = parts_of(P, b0 + lane, tokens);
-      int inc = n;
+    auto sum_up = [&](int n) {  // over this lane and those before
 #pragma unroll
       for (int s = 1; s < 32; s <<= 1) {
-        const int y = __shfl_up_sync(kFullMask, inc, s);
-        if (lane >= s) inc += y;
+        const int y = __shfl_up_sync(kFullMask, n, s);
+        if (lane >= s) n += y;
       }
-      const unsigned hit = __ballot_sync(kFullMask, at < inc);
+      return n;
+    };
+    constexpr int kMine = kSorted / 32;
+    const int* const own = groups + kMine * lane;
+    int mine = 0;
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) mine += own[k];
+    int inc = sum_up(mine);
+    unsigned hit = __ballot_sync(kFullMask, at < inc);
+    if (!hit) return false;
+    at -= inc - mine;  // into the lane's groups
+    int g = 0;
+    while (g < kMine - 1 && at >= own[g]) at -= own[g++];
+    const int owner = __ffs(hit) - 1;
+    at = __shfl_sync(kFullMask, at, owner);
+    const uint32_t group = group_of(P), b_lo = (kMine * owner + __shfl_sync(kFullMask, g, owner)) * group;
+    for (uint32_t b0 = b_lo; b0 < (uint32_t)P.batch && b0 < b_lo + group; b0 += 32) {
+      inc = sum_up(b0 + lane < (uint32_t)P.batch ? parts_of(P, b0 + lane, tokens) : 0);
+      hit = __ballot_sync(kFullMask, at < inc);
       if (hit) {
         const int w = __ffs(hit) - 1;
-        *seq = b0 + w;
+        *seq = (int)b0 + w;
         *place = __shfl_sync(kFullMask, inc, w) - 1 - at;
         return true;
       }
@@ -196,18 +231,20 @@ struct WorkList {
     }
     return false;
   }
+  template <bool MANY>
   __device__ bool find(const PromptParams& P, int index, int tokens, Work* out) const {
     const int groups = P.hq >> P.pack_log2;
     const int at = index / groups, group = index - at * groups;
     int seq, place;
-    if (!(P.batch <= kSorted ? sorted(at, &seq, &place) : in_order(P, at, tokens, &seq, &place)))
-      return false;
+    if (!(MANY ? in_order(P, at, tokens, &seq, &place) : sorted(at, &seq, &place))) return false;
     const int64_t q0 = P.cu_q[seq], nq = P.cu_q[seq + 1] - q0;
     const int64_t k0 = P.cu_kv[seq], nk = P.cu_kv[seq + 1] - k0;
     if (q0 < 0 || q0 + nq > P.total_q || k0 < 0 || nk < 0 || k0 + nk > P.total_kv) {
       if ((threadIdx.x & 31) == 0) report_device_error(P.err, FMHA_ERR_INVALID_ARG, kSitePromptLength);
       return false;
     }
+    // Where offsets that run backwards made the counts' sums overflow.
+    if (place < 0 || (int64_t)place * tokens >= nq) return false;
     out->q0 = (int)q0;
     out->nq = (int)nq;
     out->k0 = (int)k0;
@@ -335,7 +372,9 @@ __device__ __forceinline__ bool write_tile(const PromptParams& P, uint32_t o_at,
   return isnan(bad.x) || isnan(bad.y);
 }
 
-template <int D, bool BF16, bool OUT_BF16>
+// MANY: more than kSorted sequences. Its own kernel, since the registers that
+// its search takes were spilled in the softmax loop of all (2-5 %).
+template <int D, bool BF16, bool OUT_BF16, bool MANY>
 __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
     prompt_kernel(const __grid_constant__ PromptParams P) {
   using S = PromptShape<D>;
@@ -371,6 +410,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
   __shared__ __align__(16) uint4 answer;
   __shared__ uint32_t tmem_slot;
   __shared__ Work work[2];
+  __shared__ int groups[MANY ? kSorted : 1];
   __shared__ uint2 trim_at;  // the stage with rows to clear, and how many to keep
   __shared__ volatile int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -386,7 +426,12 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
   auto bar = [&](int i) { return bar0 + 8 * i; };
   const int tokens = kTileRows >> P.pack_log2;  // of a tile
   WorkList list;
-  if (warp == S::kPlanWarp) list.load(P, kTiles * tokens);
+  if constexpr (MANY) {
+    list.groups = groups;
+    list.load_groups(P, kTiles * tokens);
+  } else {
+    if (warp == S::kPlanWarp) list.load(P, kTiles * tokens);
+  }
   if (warp == S::kMmaWarp) {
     if (lane == 0) {
       abort_flag = 0;
@@ -611,7 +656,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
       bool ok = true;
       while (ok) {
         Work mine;
-        const bool found = index >= 0 && list.find(P, index, kTiles * tokens, &mine);
+        const bool found = index >= 0 && list.find<MANY>(P, index, kTiles * tokens, &mine);
         if (found || index < 0) {
           mine.last = index < 0;
           if (found) {
@@ -919,10 +964,15 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1)
 
 using PromptFn = void (*)(const PromptParams);
 
-template <int D>
+template <int D, bool MANY>
 PromptFn prompt_fn(bool bf16, bool out_bf16) {
-  if (bf16) return out_bf16 ? prompt_kernel<D, true, true> : prompt_kernel<D, true, false>;
-  return out_bf16 ? prompt_kernel<D, false, true> : prompt_kernel<D, false, false>;
+  if (bf16) return out_bf16 ? prompt_kernel<D, true, true, MANY> : prompt_kernel<D, true, false, MANY>;
+  return out_bf16 ? prompt_kernel<D, false, true, MANY> : prompt_kernel<D, false, false, MANY>;
+}
+
+template <int D>
+PromptFn prompt_fn(bool bf16, bool out_bf16, int batch) {
+  return batch > kSorted ? prompt_fn<D, true>(bf16, out_bf16) : prompt_fn<D, false>(bf16, out_bf16);
 }
 
 // The driver's tensor-map encoder, looked up once.
@@ -975,11 +1025,15 @@ extern "C" fmha_status_t fmha_prompt(const fmha_prompt_args_t* args, fmha_stream
   if (st != FMHA_OK) return st;
   if (A.dtype != FMHA_DTYPE_BF16 && A.dtype != FMHA_DTYPE_FP16) return FMHA_ERR_UNSUPPORTED;
   if (A.o_dtype != FMHA_DTYPE_BF16 && A.o_dtype != FMHA_DTYPE_FP16) return FMHA_ERR_UNSUPPORTED;
-  if (!(A.softmax_scale >= 0.0f) || std::isinf(A.softmax_scale)) return FMHA_ERR_INVALID_ARG;
+  PromptParams P;
+  std::memset(&P, 0, sizeof(P));
+  if ((st = check_scale(A.softmax_scale, d, 1.0f, &P.scale_log2)) != FMHA_OK) return st;
   if (A.total_q == 0 || A.batch == 0) return FMHA_OK;
   if ((st = check_rows(A.q, A.q_stride, hq, d)) != FMHA_OK ||
       (st = check_rows(A.o, A.o_stride, hq, d)) != FMHA_OK)
     return st;
+  // Not in place: a row that is computed again reads its query after others' outputs.
+  if (A.o == A.q) return FMHA_ERR_INVALID_ARG;
   const bool keys = A.total_kv > 0;
   if (keys && ((st = check_rows(A.k, A.k_stride, hkv, d)) != FMHA_OK ||
                (st = check_rows(A.v, A.v_stride, hkv, d)) != FMHA_OK))
@@ -992,8 +1046,6 @@ extern "C" fmha_status_t fmha_prompt(const fmha_prompt_args_t* args, fmha_stream
     return FMHA_ERR_MISALIGNED;
   ServingDevice dev;
   if ((st = serving_device(&dev)) != FMHA_OK) return st;
-  PromptParams P;
-  std::memset(&P, 0, sizeof(P));
   P.q = static_cast<const uint16_t*>(A.q);
   P.k = static_cast<const uint16_t*>(A.k);
   P.v = static_cast<const uint16_t*>(A.v);
@@ -1010,9 +1062,6 @@ extern "C" fmha_status_t fmha_prompt(const fmha_prompt_args_t* args, fmha_stream
   P.k_stride = A.k_stride;
   P.v_stride = A.v_stride;
   P.o_stride = A.o_stride;
-  const double scale =
-      A.softmax_scale > 0.0f ? (double)A.softmax_scale : 1.0 / std::sqrt((double)d);
-  P.scale_log2 = (float)(1.4426950408889634 * scale);
   P.causal = A.causal != 0;
   P.err = dev.err;
   // A wait lasts a piece at most: 15 ns a key on the tensor cores, and up to
@@ -1030,7 +1079,8 @@ extern "C" fmha_status_t fmha_prompt(const fmha_prompt_args_t* args, fmha_stream
               keys ? A.total_kv : A.total_q, keys ? A.v_stride : A.q_stride, 1, kKeys))
     return FMHA_ERR_CUDA;
   const bool out_bf16 = A.o_dtype == FMHA_DTYPE_BF16;
-  const PromptFn fn = d == 128 ? prompt_fn<128>(bf16, out_bf16) : prompt_fn<256>(bf16, out_bf16);
+  const PromptFn fn = d == 128 ? prompt_fn<128>(bf16, out_bf16, A.batch)
+                              : prompt_fn<256>(bf16, out_bf16, A.batch);
   const int smem = d == 128 ? PromptShape<128>::kSmem : PromptShape<256>::kSmem;
   const int threads = d == 128 ? PromptShape<128>::kThreads : PromptShape<256>::kThreads;
   if ((st = ensure_smem(reinterpret_cast<const void*>(fn), smem)) != FMHA_OK) return st;

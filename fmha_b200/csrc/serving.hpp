@@ -79,6 +79,14 @@ inline fmha_status_t check_cache(const fmha_paged_cache_t& in, int hkv, int d, i
   return FMHA_OK;
 }
 
+// log2(e) * the softmax scale (0: 1/sqrt(d)) * `by`.
+inline fmha_status_t check_scale(float scale, int d, float by, float* scale_log2) {
+  if (!(scale >= 0.0f) || std::isinf(scale)) return FMHA_ERR_INVALID_ARG;
+  const double s = scale > 0.0f ? (double)scale : 1.0 / std::sqrt((double)d);
+  *scale_log2 = (float)(1.4426950408889634 * s * by);
+  return *scale_log2 <= FLT_MAX ? FMHA_OK : FMHA_ERR_INVALID_ARG;
+}
+
 // Launches with programmatic stream serialization: the kernel may start while
 // the one before it in the stream finishes, and waits in
 // grid_dependency_wait() before it touches memory.

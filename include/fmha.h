@@ -183,7 +183,7 @@ fmha_status_t fmha_forward_noalloc(const void* Q, const void* K, const void* V,
  *    through fmha_device_error (FMHA_ERR_INVALID_ARG); nothing is read or
  *    written out of bounds;
  *  - softmax_scale == 0 means 1/sqrt(head_dim); a negative, NaN or infinite
- *    scale is rejected.
+ *    scale (times log2(e) and k_scale) is rejected.
  */
 
 /* Element types. */
@@ -315,7 +315,8 @@ fmha_status_t fmha_paged_decode(const fmha_paged_decode_args_t* args, fmha_strea
  * keys rows cu_seqlens_kv[b] .. cu_seqlens_kv[b+1]-1 (device int32
  * [batch+1]; cu_seqlens_kv null: the same as cu_seqlens_q). With `causal`,
  * query i of nq sees keys j <= i + (nk - nq): the last query sees every key.
- * Rows behind the last sequence are left as they were.
+ * Rows behind the last sequence are left as they were. O must not overlap Q,
+ * K or V.
  */
 typedef struct fmha_prompt_args {
   const void* q;

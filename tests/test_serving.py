@@ -87,7 +87,8 @@ def test_append_refuses(kw, status):
 @pytest.mark.parametrize("kw,status", HEADS + PAGES + [
     (dict(o=0), INVALID), (dict(o=36), MISALIGNED), (dict(o_stride=4000), INVALID), (dict(lse=66), MISALIGNED),
     (dict(o_dtype=E4M3), UNSUPPORTED), (dict(softmax_scale=-1.0), INVALID), (dict(softmax_scale=NAN), INVALID),
-    (dict(softmax_scale=INF), INVALID), (dict(workspace=0), INVALID), (dict(workspace=(1 << 12) + 8), MISALIGNED),
+    (dict(softmax_scale=INF), INVALID), (dict(softmax_scale=3e38), INVALID),
+    (dict(workspace=0), INVALID), (dict(workspace=(1 << 12) + 8), MISALIGNED),
     (dict(workspace_bytes=1000), INVALID), (dict(batch=1 << 28), UNSUPPORTED),
 ])
 def test_decode_refuses(kw, status):
@@ -101,6 +102,7 @@ def test_decode_refuses(kw, status):
     (dict(cu_seqlens_q=0), INVALID), (dict(cu_seqlens_q=130), MISALIGNED), (dict(cu_seqlens_kv=131), MISALIGNED),
     (dict(total_kv=10), INVALID), (dict(o_dtype=E4M3), UNSUPPORTED), (dict(softmax_scale=-0.5), INVALID),
     (dict(softmax_scale=NAN), INVALID), (dict(o_stride=1 << 31), UNSUPPORTED),
+    (dict(softmax_scale=3e38), INVALID), (dict(o=16), INVALID),
 ])
 def test_prompt_refuses(kw, status):
     assert prompt(**kw) == status

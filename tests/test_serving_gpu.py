@@ -538,6 +538,42 @@ def test_prompt_many_sequences(cuda, b):
     prompt_case(nq, [n + i % 3 for i, n in enumerate(nq)], 4, 2, 128, BF16, BF16, True, seed=b)
 
 
+@pytest.mark.parametrize("b,d,hq,out", [(257, 128, 4, BF16), (1000, 256, 8, FP16), (8193, 128, 2, FP16)])
+def test_prompt_is_the_same_in_one_call_or_many(cuda, b, d, hq, out):
+    """Sequences do not depend on their neighbours: bit for bit what calls of 100 give."""
+    g = gen(b)
+    nq = [(5 * i) % 4 if i % 301 else 400 for i in range(b)]
+    q, k, v = (randn((sum(nq), h, d), g, BF16) for h in (hq, 2, 2))
+    o = fmha_b200.fmha_prompt(q, k, v, starts(nq), out_dtype=out)
+    at = 0
+    for i in range(0, b, 100):
+        part = nq[i:i + 100]
+        rows = slice(at, at + sum(part))
+        at += sum(part)
+        if sum(part):
+            want = fmha_b200.fmha_prompt(q[rows], k[rows], v[rows], starts(part), out_dtype=out)
+            assert torch.equal(bits(o[rows]), bits(want)), i
+    assert fmha_b200.device_error() == 0
+
+
+def test_prompt_leaves_out_impossible_ones_of_many(cuda):
+    """Offsets that run back or past the rows, among more sequences than are sorted."""
+    g = gen(26)
+    b, n, hq, d = 600, 3, 4, 128
+    q, k, v = (randn((b * n, h, d), g, BF16) for h in (hq, 2, 2))
+    want = fmha_b200.fmha_prompt(q[:300], k[:300], v[:300], starts([n] * 100))
+    for bad in (-2 ** 31, -1, 0, 2 ** 31 - 1):
+        cu = starts([n] * b)
+        cu[350:] = bad
+        o = torch.full((b * n, hq, d), 7.0, dtype=FP16, device="cuda")
+        fmha_b200.fmha_prompt(q, k, v, cu, o=o)
+        torch.cuda.synchronize()
+        assert error_site() == (fmha_b200.FMHA_ERR_INVALID_ARG, SITE_PROMPT_LENGTH)
+        assert torch.equal(bits(o[:300]), bits(want))
+        assert bool((o[349 * n:] == 7.0).all())
+    assert fmha_b200.device_error() == 0
+
+
 @pytest.mark.parametrize("d,dtype,out", [(128, BF16, BF16), (128, BF16, FP16), (256, FP16, FP16), (256, BF16, BF16)])
 def test_prompt_repeats(cuda, d, dtype, out):
     """Many short and long pieces in a row, on and on: the same bits every time, and no wait
