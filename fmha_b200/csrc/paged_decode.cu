@@ -21,13 +21,14 @@
 // by a power of two that puts its largest element just below 2^15.
 //
 // Split. A unit is one (sequence, kv head, up to 16 of its query heads); a
-// tile is 16 of its tokens (32 of an e4m3 cache at head_dim 128). All tiles of all units, one
-// after the other, are dealt out in equal contiguous ranges to the CTAs and
-// within them to the warps, whatever the lengths, so ragged batches and a
-// single long sequence fill the card alike. A unit counts one tile more than
-// it has, for its query's load and its output. Each CTA finds its ranges from
-// a prefix sum over the lengths, which are only known on the device; a
-// captured launch therefore stays right as sequences grow. A warp writes the
+// tile is 16 of its tokens (32 of an e4m3 cache at head_dim 128). All tiles
+// of all units, one after the other, are dealt out in equal contiguous ranges
+// to the CTAs and within them to the warps, whatever the lengths, so ragged
+// batches and a single long sequence fill the card alike. A unit counts one
+// tile more than it has, for its query's load and its output. The ranges come
+// from a prefix sum over the lengths, which are only known on the device (by
+// each warp alone for up to kFew sequences, else by the CTA); a captured
+// launch therefore stays right as sequences grow. A warp writes the
 // outputs of units that begin and end in its range; the at most two others
 // wait in shared memory until the CTA's warps are done and are joined there.
 // A unit that crosses from one CTA into the next leaves a partial result in
@@ -94,10 +95,9 @@ struct DecodeShape {
   static constexpr int kChunks = kRowBytes / 16;  // 16-byte pieces of a row
   // 16-token steps of a tile, warps, and tiles of a warp's ring. e4m3 tiles
   // cost twice the instructions per byte, so the warps' latency shows first:
-  // at head_dim 128 two steps at a time overlap (5.3 TB/s, 128 sequences of
-  // 2048 tokens, 32/8 heads; one step 4.3, 12 warps 4.8), at 256 eight warps
-  // (5.5 TB/s, 64 of 4096, 32/16 heads; 4 warps with two steps 4.4, 7 with a
-  // longer ring 4.8).
+  // at head_dim 128 two steps at a time overlap (5.65 TB/s, 128 sequences of
+  // 2048 tokens, 32/8 heads; one step 4.72), at 256 eight warps do (6.24 TB/s,
+  // 64 of 4096, 32/16 heads; 4 warps with two steps 4.89).
   static constexpr int kSub = F8 && D == 128 ? 2 : 1;
   static constexpr int kTile = 16 * kSub;
   static constexpr int kRows = WIDE ? 16 : 8;
