@@ -14,8 +14,9 @@ adjacent D, so a pool stored token by token is passed as
 ``pool.transpose(1, 2)``. Head dimension 128 or 256; q, k and v bf16 or fp16;
 pages of the same type, or float8_e4m3fn with a scale. The calls run on
 torch's current stream of q's device (or ``stream``), allocate their outputs
-and workspace there, and raise FmhaError for arguments that they refuse. The
-checks are in csrc/serving_py.cpp.
+and workspace there, and raise FmhaError for arguments that they refuse. They
+are for inference: outputs carry no gradient. The checks are in
+csrc/serving_py.cpp.
 """
 from __future__ import annotations
 
